@@ -90,6 +90,16 @@ SIGNATURES = {
     "jirf_train_window_attention": (_i, [_fp, _l, _fp, _fp, _fp, _l, _i, _i, _i, _i, _i, _i, _i, _vp]),
     "jirf_train_window_attention_bwd": (_i, [_fp, _l, _fp, _fp, _fp, _l, _fp, _l, _fp, _fp, _i, _i, _i, _i, _i, _i, _i,
                                              _i, _vp]),
+    "jirf_train_residual_norm": (_i, [_vp, _l, _vp, _l, _i, _i, _i, _fp, _fp, _i, _fp, _fp, _i, _fp, _fp, C.c_float, _vp, _l, _vp,
+                                      _l, _fp, _i, _i, _i, _vp]),
+    "jirf_train_residual_norm_bwd_work_floats": (_l, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "jirf_train_residual_norm_bwd": (_i, [_vp, _l, _vp, _l, _vp, _l, _vp, _l, _fp, _i, _i, _i, _fp, _fp, _i, _fp, _fp, _i, _fp,
+                                          _vp, _l, _vp, _l, _fp, _fp, _fp, _fp, _fp, _i, _fp, _i, _i, _i, _vp]),
+    "jirf_train_grad_clip_plan_create": (_i, [_i, C.POINTER(_vp), C.POINTER(_i), C.POINTER(_vp), C.POINTER(_i), C.POINTER(_l),
+                                              C.POINTER(_vp)]),
+    "jirf_train_grad_clip_work_doubles": (_l, [_vp]),
+    "jirf_train_grad_clip_run": (_i, [_vp, _i, C.c_double, C.c_double, _vp, _vp, _vp]),
+    "jirf_train_grad_clip_plan_destroy": (None, [_vp]),
     "jirf_op_gelu_error_scan": (_i, [C.c_float, C.POINTER(C.c_double), _vp]),
     "jirf_set_gemm_split_bf16": (_i, [_i]),
     "jirf_op_conv3x3": (_i, [_fp, _vp, _vp, _fp, _fp, _i, _i, _i, _i, _i, _i, _vp]),

@@ -43,6 +43,9 @@ typedef struct jirf_net jirf_net;
 #define JIRF_I32 1
 #define JIRF_I64 2
 #define JIRF_F64 3
+/* further dtype tags: activations and gradients of jirf_train_residual_norm* and jirf_train_grad_clip* */
+#define JIRF_BF16 4
+#define JIRF_F16 5
 
 /* batch semantics of jirf_net_forward for B > 1 */
 #define JIRF_BATCH_PER_IMAGE 0 /* equals B separate B=1 reference calls (what every test script does) */
@@ -436,6 +439,65 @@ int jirf_train_window_attention(const float* qkv, long qkv_bs, const float* tabl
 int jirf_train_window_attention_bwd(const float* qkv, long qkv_bs, const float* table, const float* w2, const float* dout,
                                     long dout_bs, float* dqkv, long dqkv_bs, float* dtable, float* dw2, int B, int C, int H,
                                     int W, int heads, int shift, int coupled, int accumulate, void* stream);
+
+/* The join of a residual block with the norms on both sides of it, in one pass over the activations:
+ *     u = N_post(f) (or f);   y = x + scale[b] * gate * u;   n = N_pre(y) (or no n)
+ * what jirf_train_scale_add followed by jirf_train_layernorm computes (a branch under stochastic depth and the norm of
+ * the next branch, ast_arch.py:786-842), with an optional norm after the branch and an optional gate.
+ *   dtype      JIRF_F32, JIRF_BF16 or JIRF_F16, for every activation; the arithmetic is fp32, each stored value rounded
+ *              once (n is formed from the fp32 sum, not from the rounded y)
+ *   layout     JIRF_LAYOUT_PLANAR [B][C][P] or JIRF_LAYOUT_TOKENS [B][P][C] (the reference's token order); batch strides
+ *              in elements, 0 = dense, the C * P elements of an image contiguous
+ *   post_kind, pre_kind   0 none, 1 LayerNorm (bias or NULL), 2 BiasFree, 3 root mean square; over the channels
+ *   gate_kind  0 none, 1 gate [C], 2 gate [B][C];   scale [B] or NULL
+ *   stats      NULL, or [4][B][P] for the backward: mean and reciprocal deviation of f, then of y (0 where there is no
+ *              norm; mean 0 for kind 3)
+ * Parameters, gate, scale and stats are fp32.  y may be x and n may be f; other outputs overlap nothing. */
+#define JIRF_LAYOUT_PLANAR 0
+#define JIRF_LAYOUT_TOKENS 1
+int jirf_train_residual_norm(const void* x, long x_bs, const void* f, long f_bs, int dtype, int layout, int post_kind,
+                             const float* post_w, const float* post_b, int gate_kind, const float* gate, const float* scale,
+                             int pre_kind, const float* pre_w, const float* pre_b, float eps, void* y, long y_bs, void* n,
+                             long n_bs, float* stats, int B, int C, int P, void* stream);
+/* Its backward.  dy (or NULL: zero) is the gradient arriving over the residual stream, dn that of n; y and stats are the
+ * forward's, f its branch input (NULL where neither norm nor gate sits on the branch; dn, y NULL without N_pre).
+ *     dx = dy + dN_pre(dn),   df = dN_post(scale * gate * dx)
+ * and the parameter gradients dpost_w, dpost_b, dpre_w, dpre_b [C], dgate [C] or [B][C], each NULL when not wanted,
+ * accumulate != 0 adds to them.  No gradient for scale (it is drawn, not learned).  work: DEVICE memory of
+ * jirf_train_residual_norm_bwd_work_floats() floats owned by the caller, needed only during the call (calls that
+ * run at the same time need one each); that function returns < 0 for bad arguments.  Outputs overlap nothing.
+ * Sums have a fixed order (no atomics). */
+long jirf_train_residual_norm_bwd_work_floats(int dtype, int layout, int post_kind, int gate_kind, int pre_kind, int B, int C,
+                                              int P);
+int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, long dn_bs, const void* y, long y_bs, const void* f,
+                                 long f_bs, const float* stats, int dtype, int layout, int post_kind, const float* post_w,
+                                 const float* post_b, int gate_kind, const float* gate, const float* scale, int pre_kind,
+                                 const float* pre_w, void* dx, long dx_bs, void* df, long df_bs, float* dpost_w, float* dpost_b,
+                                 float* dgate, float* dpre_w, float* dpre_b, int accumulate, float* work, int B, int C, int P,
+                                 void* stream);
+
+/* Optimizer.clip_grad_norm (image_restoration_model.py:269-270) over many separate tensors, as the reference's optimizer
+ * holds its gradients (jirf_train_sumsq / jirf_train_adam_step do it for one flat buffer):
+ *     total = grad_scale * (sum g^2)^(1/2)  [JIRF_NORM_L2]   or   grad_scale * max |g|  [JIRF_NORM_MAX]
+ *     k = grad_scale * min(max_norm / (total + 1e-6), 1)   (max_norm <= 0: k = grad_scale);   dst = k * g
+ * A plan lists n tensors once: src[i] of count[i] contiguous elements (0 allowed) and src_dtype[i], and dst[i] with
+ * dst_dtype[i] - its own source (in place; same dtype size) or other memory that no other tensor touches, of any of the three
+ * types, e.g. slices of the flat fp32 buffer of jirf_train_adam_step - or dst NULL: norm only.  The plan belongs to
+ * the device current at creation, holds the addresses, is not changed by a run, and must outlive every queued run and
+ * captured graph that uses it; make and destroy it outside stream captures.
+ * A run writes stats [3] (DEVICE, float64): the sum of squares (what jirf_train_adam_step takes) or the maximum
+ * as stored, total, and k; it is asynchronous and can be captured.  A NaN among the gradients gives NaN for all three, an
+ * infinity total = inf and k = 0 (0 for finite gradients, NaN for the infinite ones), as the formulas do.  work: DEVICE
+ * memory of jirf_train_grad_clip_work_doubles() float64 owned by the caller, needed only during the run (runs at the same
+ * time need one each).  All sums are 64-bit in a fixed order. */
+#define JIRF_NORM_L2 0
+#define JIRF_NORM_MAX 1
+int jirf_train_grad_clip_plan_create(int n, const void* const* src, const int* src_dtype, void* const* dst,
+                                     const int* dst_dtype, const long* count, void** plan_out);
+long jirf_train_grad_clip_work_doubles(const void* plan);
+int jirf_train_grad_clip_run(const void* plan, int norm_kind, double max_norm, double grad_scale, double* stats, double* work,
+                             void* stream);
+void jirf_train_grad_clip_plan_destroy(void* plan);
 
 #ifdef __cplusplus
 }

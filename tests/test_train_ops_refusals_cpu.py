@@ -1,0 +1,113 @@
+"""What the residual norm and the gradient clip refuse, on the host: the library's argument checks return before any
+launch, so no GPU is needed (addresses are made up and never read), and the Python layer's raise before the library."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import jirf_hip
+from jirf_hip import train_ops as T
+
+A, B_, D, E = (0x1000_0000 * i for i in (1, 2, 3, 4))      # four far apart, aligned addresses
+EINVAL = -1
+
+
+def fwd(**kw):
+    a = dict(x=A, x_bs=0, f=B_, f_bs=0, dtype=0, layout=0, post=0, post_w=None, post_b=None, gate_kind=0, gate=None, scale=None,
+             pre=0, pre_w=None, pre_b=None, eps=1e-5, y=D, y_bs=0, n=None, n_bs=0, stats=None, B=2, C=8, P=16, stream=None)
+    assert not set(kw) - set(a)
+    a.update(kw)
+    return jirf_hip.lib().jirf_train_residual_norm(*a.values())
+
+
+def bwd(**kw):
+    a = dict(dy=A, dy_bs=0, dn=None, dn_bs=0, y=None, y_bs=0, f=None, f_bs=0, stats=None, dtype=0, layout=0, post=0, post_w=None,
+             post_b=None, gate_kind=0, gate=None, scale=None, pre=0, pre_w=None, dx=D, dx_bs=0, df=E, df_bs=0, dpost_w=None,
+             dpost_b=None, dgate=None, dpre_w=None, dpre_b=None, accumulate=0, work=None, B=2, C=8, P=16, stream=None)
+    assert not set(kw) - set(a)
+    a.update(kw)
+    return jirf_hip.lib().jirf_train_residual_norm_bwd(*a.values())
+
+
+BAD_COMMON = [dict(dtype=1), dict(dtype=3), dict(dtype=6), dict(dtype=-1), dict(layout=2), dict(layout=-1), dict(post=4, post_w=A),
+              dict(post=-1), dict(pre=4, pre_w=A), dict(gate_kind=3, gate=A), dict(gate_kind=-1), dict(B=0), dict(C=0), dict(P=0),
+              dict(B=-1), dict(gate_kind=1), dict(gate_kind=2)]
+
+
+@pytest.mark.parametrize("kw", BAD_COMMON + [
+    dict(x=None), dict(f=None), dict(y=None), dict(post=1), dict(pre=1, n=E), dict(pre=1, pre_w=A), dict(eps=-1.0), dict(eps=math.nan),
+    dict(eps=math.inf), dict(x_bs=127), dict(y_bs=-128), dict(f_bs=1), dict(x=A + 2), dict(dtype=4, f=B_ + 1), dict(y=D + 1),
+    dict(pre=1, pre_w=A, n=E, n_bs=100), dict(y=A + 64), dict(y=B_), dict(pre=3, pre_w=A, n=D), dict(pre=3, pre_w=A, n=A)])
+def test_forward_refuses(kw):
+    assert fwd(**kw) == EINVAL and "residual_norm" in jirf_hip.last_error()
+
+
+@pytest.mark.parametrize("kw", BAD_COMMON + [
+    dict(dx=None), dict(df=None), dict(dy=None), dict(pre=1, pre_w=A, y=B_, stats=B_, work=A), dict(pre=1, pre_w=A, dn=B_, stats=B_, work=A),
+    dict(pre=1, pre_w=A, dn=B_, y=B_, work=A), dict(pre=1, dn=B_, y=B_, stats=B_, work=A), dict(post=1, post_w=A, stats=B_, work=A),
+    dict(gate_kind=1, gate=A, work=A), dict(post=2, post_w=A, f=B_, work=A), dict(dpost_w=A, work=A), dict(dgate=A, work=A),
+    dict(dpre_w=A, work=A), dict(dpre_b=A, work=A), dict(post=2, post_w=A, f=B_, stats=B_, dpost_b=A, work=A),
+    dict(pre=3, pre_w=A, dn=B_, y=B_, stats=B_, dpre_b=A, work=A), dict(gate_kind=1, gate=A, f=B_, dgate=A), dict(dy_bs=5),
+    dict(dx_bs=127), dict(df_bs=-3), dict(dx=D + 1), dict(df=D), dict(dx=A), dict(df=A + 256)])
+def test_backward_refuses(kw):
+    assert bwd(**kw) == EINVAL and "residual_norm_bwd" in jirf_hip.last_error()
+
+
+def test_backward_work_size():
+    size = jirf_hip.lib().jirf_train_residual_norm_bwd_work_floats
+    assert size(0, 0, 1, 2, 1, 2, 64, 1000) > 0
+    for bad in ((1, 0, 0, 0, 0, 1, 1, 1), (0, 2, 0, 0, 0, 1, 1, 1), (0, 0, 4, 0, 0, 1, 1, 1), (0, 0, 0, 3, 0, 1, 1, 1),
+                (0, 0, 0, 0, 5, 1, 1, 1), (0, 0, 0, 0, 0, 0, 1, 1), (0, 0, 0, 0, 0, 1, -1, 1), (0, 0, 0, 0, 0, 1, 1, 0)):
+        assert size(*bad) < 0, bad
+
+
+def plan(src, sdt, dst, ddt, count, n=None):
+    n = len(src) if n is None else n
+    k = max(1, len(src))
+    out = C.c_void_p()
+    rc = jirf_hip.lib().jirf_train_grad_clip_plan_create(
+        n, (C.c_void_p * k)(*src), (C.c_int * k)(*sdt), None if dst is None else (C.c_void_p * k)(*dst),
+        None if ddt is None else (C.c_int * k)(*ddt), (C.c_long * k)(*count), C.byref(out))
+    assert rc != 0 and not out.value
+    return rc
+
+
+@pytest.mark.parametrize("args", [
+    ([], [], None, None, []),                                                # no tensors
+    ([A], [1], None, None, [4]), ([A], [0], [D], [3], [4]), ([A], [9], None, None, [4]),          # types
+    ([None], [0], None, None, [4]), ([A], [0], [None], [0], [4]), ([A], [0], None, None, [-1]),   # addresses, sizes
+    ([A], [0], [D], None, [4]),                                              # destinations without types
+    ([A + 1], [4], None, None, [4]), ([A + 2], [0], None, None, [4]), ([A], [0], [D + 2], [0], [4]), ([A], [0], [D + 1], [4], [4]),
+    ([A, B_], [0, 0], [D, D], [0, 0], [4, 4]), ([A, B_], [0, 0], [D, D + 12], [0, 0], [4, 4]),    # overlapping destinations
+    ([A, B_], [0, 0], [D, A], [0, 0], [4, 4]), ([A, A], [0, 0], [A, D], [0, 0], [4, 4]),          # onto another's source
+    ([A], [0], [A + 4], [0], [4]), ([A], [0], [A], [4], [4]), ([A, A], [0, 0], [A, A], [0, 0], [4, 4]),   # onto a part of itself
+    ([A, D], [0, 0], [B_, E], [0, 0], [0x1000_0000, 4]),                     # a long one across its neighbours
+])
+def test_clip_plan_refuses(args):
+    assert plan(*args) == EINVAL and "grad_clip" in jirf_hip.last_error()
+
+
+def test_clip_run_refuses_null():
+    L = jirf_hip.lib()
+    assert L.jirf_train_grad_clip_run(None, 0, 1.0, 1.0, A, A, None) == EINVAL
+    assert L.jirf_train_grad_clip_work_doubles(None) < 0
+    L.jirf_train_grad_clip_plan_destroy(None)
+
+
+def test_python_layer_refuses():
+    x = torch.zeros(2, 8, 4)
+    with pytest.raises(ValueError, match="no CPU path"):
+        T.residual_norm(x, x)
+    with pytest.raises(ValueError, match="layout"):
+        T.residual_norm(x, x, layout="rows")
+    with pytest.raises(ValueError, match="dy or dn"):
+        T.residual_norm_bwd(None, None, None, None, None)
+    with pytest.raises(ValueError, match="no CPU path"):
+        T.residual_norm_bwd(x, None, None, None, None)
+    with pytest.raises(ValueError, match="no tensors"):
+        T.GradientClip([])
+    with pytest.raises(ValueError, match="one GPU"):
+        T.GradientClip([x])
+    with pytest.raises(ValueError, match="2 tensors, 1 outputs"):
+        T.GradientClip([x, x], out=[x])
