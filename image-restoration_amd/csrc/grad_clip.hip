@@ -23,8 +23,9 @@
 namespace jirf {
 namespace {
 
-constexpr int CLIP_T = 256;            // threads per workgroup
-constexpr int CLIP_E = 8;              // elements per thread and step
+constexpr int CLIP_T = 256;            // threads that share a chunk
+constexpr int CLIP_E = 8;              // elements per thread and access
+constexpr int CLIP_U = 4;              // accesses of one thread in flight
 constexpr int CLIP_MAX_BLOCKS = 2048;  // eight workgroups per CU
 enum { TY_F32 = 0, TY_BF16 = 1, TY_F16 = 2 };
 
@@ -35,90 +36,235 @@ struct ClipChunk {
   unsigned types;         // source type | destination type << 8
 };
 
-__device__ __forceinline__ float clip_load(const void* p, unsigned ty, long i) {
-  if (ty == TY_F32) return static_cast<const float*>(p)[i];
-  if (ty == TY_BF16) return __uint_as_float((unsigned)static_cast<const uint16_t*>(p)[i] << 16);
-  return (float)static_cast<const _Float16*>(p)[i];
+// Eight consecutive elements, 16 bytes per access, at the alignment of one element (a tensor packed tight between others
+// starts anywhere; the memory instructions take any 4- or 2-byte address).
+typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <int TY>
+struct Raw {              // eight elements as loaded
+  u32x4 a, b;             // b: fp32 only
+};
+template <int TY>
+__device__ __forceinline__ Raw<TY> clip_load8(const void* p, unsigned g) {
+  Raw<TY> r{};
+  if constexpr (TY == TY_F32) {
+    const u32x4_a4* q = reinterpret_cast<const u32x4_a4*>(static_cast<const float*>(p) + (size_t)g * CLIP_E);
+    r.a = q[0];
+    r.b = q[1];
+  } else {
+    r.a = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(p) + (size_t)g * CLIP_E);
+  }
+  return r;
 }
-// round to nearest even, NaN kept quiet
-__device__ __forceinline__ uint16_t to_bf16(float v) {
-  return __builtin_bit_cast(uint16_t, (__bf16)v);
+template <int TY>
+__device__ __forceinline__ f32x8 clip_widen(const Raw<TY>& r) {
+  f32x8 v;
+  if constexpr (TY == TY_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __uint_as_float(r.a[i]);
+      v[4 + i] = __uint_as_float(r.b[i]);
+    }
+  } else if constexpr (TY == TY_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(r.a[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r.a[i] & 0xffff0000u);
+    }
+  } else {
+    const f16x8 h = __builtin_bit_cast(f16x8, r.a);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+  }
+  return v;
 }
-__device__ __forceinline__ void clip_store(void* p, unsigned ty, long i, float v) {
-  if (ty == TY_F32) static_cast<float*>(p)[i] = v;
-  else if (ty == TY_BF16) static_cast<uint16_t*>(p)[i] = to_bf16(v);
+// rounded to nearest even
+template <int TY>
+__device__ __forceinline__ void clip_store8(void* p, unsigned g, const f32x8& v) {
+  if constexpr (TY == TY_F32) {
+    u32x4_a4* q = reinterpret_cast<u32x4_a4*>(static_cast<float*>(p) + (size_t)g * CLIP_E);
+    u32x4 a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = __float_as_uint(v[i]);
+      b[i] = __float_as_uint(v[4 + i]);
+    }
+    q[0] = a;
+    q[1] = b;
+  } else if constexpr (TY == TY_BF16) {
+    bf16x8 h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (__bf16)v[i];
+    *reinterpret_cast<u32x4_a2*>(static_cast<uint16_t*>(p) + (size_t)g * CLIP_E) = __builtin_bit_cast(u32x4, h);
+  } else {
+    f16x8 h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i];
+    *reinterpret_cast<u32x4_a2*>(static_cast<uint16_t*>(p) + (size_t)g * CLIP_E) = __builtin_bit_cast(u32x4, h);
+  }
+}
+template <int TY>
+__device__ __forceinline__ float clip_load1(const void* p, unsigned i) {
+  if constexpr (TY == TY_F32) return static_cast<const float*>(p)[i];
+  else if constexpr (TY == TY_BF16) return __uint_as_float((unsigned)static_cast<const uint16_t*>(p)[i] << 16);
+  else return (float)static_cast<const _Float16*>(p)[i];
+}
+template <int TY>
+__device__ __forceinline__ void clip_store1(void* p, unsigned i, float v) {
+  if constexpr (TY == TY_F32) static_cast<float*>(p)[i] = v;
+  else if constexpr (TY == TY_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
   else static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 // A maximum that a NaN wins: the bit patterns of |v| order like the values, with every NaN above infinity.
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
-template <bool MAX>
-__device__ __forceinline__ double block_combine(double v, double* red) {
-  const int tid = threadIdx.x;
-  red[tid] = v;
-  __syncthreads();
-  for (int s = CLIP_T / 2; s > 0; s >>= 1) {
-    if (tid < s) {
-      const double o = red[tid + s];
-      if (MAX) red[tid] = (o > red[tid] || o != o) ? o : red[tid];
-      else red[tid] += o;
+struct ClipAcc {
+  double sum = 0.0;
+  unsigned mx = 0;
+};
+
+// One chunk's share of thread `t` of CLIP_T.
+template <bool MAX, int TY>
+__device__ __forceinline__ void norm_chunk(const ClipChunk& ck, unsigned t, ClipAcc& acc) {
+  const unsigned groups = ck.n / CLIP_E;
+  auto add = [&](const Raw<TY>& r) {
+    const f32x8 v = clip_widen<TY>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (MAX) acc.mx = max(acc.mx, abs_bits(v[i]));
+      else acc.sum = fma((double)v[i], (double)v[i], acc.sum);
     }
-    __syncthreads();
+  };
+  unsigned g = t;
+  for (; g + (CLIP_U - 1) * CLIP_T < groups; g += CLIP_U * CLIP_T) {
+    Raw<TY> r[CLIP_U];
+#pragma unroll
+    for (int u = 0; u < CLIP_U; ++u) r[u] = clip_load8<TY>(ck.src, g + u * CLIP_T);
+#pragma unroll
+    for (int u = 0; u < CLIP_U; ++u) add(r[u]);
   }
-  const double r = red[0];
+  for (; g < groups; g += CLIP_T) add(clip_load8<TY>(ck.src, g));
+  const unsigned i = groups * CLIP_E + t;
+  if (i < ck.n) {
+    const float v = clip_load1<TY>(ck.src, i);
+    if (MAX) acc.mx = max(acc.mx, abs_bits(v));
+    else acc.sum = fma((double)v, (double)v, acc.sum);
+  }
+}
+template <bool MAX>
+__device__ __forceinline__ void norm_any(const ClipChunk& ck, unsigned t, ClipAcc& acc) {
+  const unsigned ty = ck.types & 0xff;
+  if (ty == TY_F32) norm_chunk<MAX, TY_F32>(ck, t, acc);
+  else if (ty == TY_BF16) norm_chunk<MAX, TY_BF16>(ck, t, acc);
+  else norm_chunk<MAX, TY_F16>(ck, t, acc);
+}
+
+template <int TS, int TD>
+__device__ __forceinline__ void scale_chunk(const ClipChunk& ck, unsigned t, float k) {
+  const unsigned groups = ck.n / CLIP_E;
+  unsigned g = t;
+  for (; g + (CLIP_U - 1) * CLIP_T < groups; g += CLIP_U * CLIP_T) {
+    Raw<TS> r[CLIP_U];
+#pragma unroll
+    for (int u = 0; u < CLIP_U; ++u) r[u] = clip_load8<TS>(ck.src, g + u * CLIP_T);
+#pragma unroll
+    for (int u = 0; u < CLIP_U; ++u) clip_store8<TD>(ck.dst, g + u * CLIP_T, clip_widen<TS>(r[u]) * k);
+  }
+  for (; g < groups; g += CLIP_T) clip_store8<TD>(ck.dst, g, clip_widen<TS>(clip_load8<TS>(ck.src, g)) * k);
+  const unsigned i = groups * CLIP_E + t;
+  if (i < ck.n) clip_store1<TD>(ck.dst, i, clip_load1<TS>(ck.src, i) * k);
+}
+template <int TS>
+__device__ __forceinline__ void scale_to(const ClipChunk& ck, unsigned t, float k) {
+  const unsigned td = ck.types >> 8;
+  if (td == TY_F32) scale_chunk<TS, TY_F32>(ck, t, k);
+  else if (td == TY_BF16) scale_chunk<TS, TY_BF16>(ck, t, k);
+  else scale_chunk<TS, TY_F16>(ck, t, k);
+}
+__device__ __forceinline__ void scale_any(const ClipChunk& ck, unsigned t, float k) {
+  const unsigned ts = ck.types & 0xff;
+  // in place with factor 1 every value stays as it is
+  if (k == 1.0f && ck.src == ck.dst && ts == ck.types >> 8) return;
+  if (ts == TY_F32) scale_to<TY_F32>(ck, t, k);
+  else if (ts == TY_BF16) scale_to<TY_BF16>(ck, t, k);
+  else scale_to<TY_F16>(ck, t, k);
+}
+
+// Combines over the workgroup (butterfly in each wave, then the waves in order); the result in every thread.
+template <bool MAX>
+__device__ __forceinline__ double combine2(double a, double b) {
+  if (MAX) return (b > a || b != b) ? b : a;
+  return a + b;
+}
+template <bool MAX, int T>
+__device__ __forceinline__ double block_combine(double v, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = combine2<MAX>(v, __shfl_xor(v, o));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
+  double r = red[0];
+#pragma unroll
+  for (int w = 1; w < T / 64; ++w) r = combine2<MAX>(r, red[w]);
   return r;
 }
 
 template <bool MAX>
-__global__ __launch_bounds__(CLIP_T) void norm_kernel(const ClipChunk* __restrict__ chunks, int n_chunks,
-                                                      double* __restrict__ part) {
-  __shared__ double red[CLIP_T];
-  double acc = 0.0;
-  unsigned mx = 0;
-  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
-    const ClipChunk ck = chunks[c];
-    const unsigned ty = ck.types & 0xff;
-    for (unsigned i = threadIdx.x; i < ck.n; i += CLIP_T) {
-      const float g = clip_load(ck.src, ty, i);
-      if (MAX) mx = max(mx, abs_bits(g));
-      else acc = fma((double)g, (double)g, acc);
-    }
-  }
-  const double r = block_combine<MAX>(MAX ? (double)__uint_as_float(mx) : acc, red);
-  if (threadIdx.x == 0) part[blockIdx.x] = r;
-}
-
-template <bool MAX>
-__global__ __launch_bounds__(CLIP_T) void clip_kernel(const ClipChunk* __restrict__ chunks, int n_chunks,
-                                                      const double* __restrict__ part, int n_part, double max_norm,
-                                                      double grad_scale, double* __restrict__ stats) {
-  __shared__ double red[CLIP_T];
-  double t = 0.0;
-  for (int i = threadIdx.x; i < n_part; i += CLIP_T) {
-    const double o = part[i];
-    if (MAX) t = (o > t || o != o) ? o : t;
-    else t += o;
-  }
-  const double raw = block_combine<MAX>(t, red);
+__device__ __forceinline__ float clip_factor(double raw, double max_norm, double grad_scale, double* stats, bool write) {
   const double total = grad_scale * (MAX ? raw : sqrt(raw));
   double k = grad_scale;
   if (max_norm > 0.0) {
     const double c = max_norm / (total + 1e-6);
     k *= c >= 1.0 ? 1.0 : c;           // a NaN norm gives NaN, as the formula does
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  if (write) {
     stats[0] = raw;
     stats[1] = total;
     stats[2] = k;
   }
-  const float kf = (float)k;
-  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
-    const ClipChunk ck = chunks[c];
-    if (!ck.dst) continue;
-    const unsigned ty = ck.types & 0xff, td = ck.types >> 8;
-    for (unsigned i = threadIdx.x; i < ck.n; i += CLIP_T) clip_store(ck.dst, td, i, clip_load(ck.src, ty, i) * kf);
-  }
+  return (float)k;
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(CLIP_T) void norm_kernel(const ClipChunk* __restrict__ chunks, int n_chunks,
+                                                      double* __restrict__ part) {
+  __shared__ double red[CLIP_T / 64];
+  ClipAcc acc;
+  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) norm_any<MAX>(chunks[c], threadIdx.x, acc);
+  const double r = block_combine<MAX, CLIP_T>(MAX ? (double)__uint_as_float(acc.mx) : acc.sum, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = r;
+}
+
+// The chunks are taken from the last to the first: what norm_kernel read last is what the cache still holds.
+template <bool MAX>
+__global__ __launch_bounds__(CLIP_T) void clip_kernel(const ClipChunk* __restrict__ chunks, int n_chunks,
+                                                      const double* __restrict__ part, int n_part, double max_norm,
+                                                      double grad_scale, double* __restrict__ stats) {
+  __shared__ double red[CLIP_T / 64];
+  double t = 0.0;
+  for (int i = threadIdx.x; i < n_part; i += CLIP_T) t = combine2<MAX>(t, part[i]);
+  const double raw = block_combine<MAX, CLIP_T>(t, red);
+  const float k = clip_factor<MAX>(raw, max_norm, grad_scale, stats, blockIdx.x == 0 && threadIdx.x == 0);
+  for (int c = n_chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) scale_any(chunks[c], threadIdx.x, k);
+}
+
+// Few chunks: one workgroup of four chunk teams does both passes in one launch.
+constexpr int CLIP_SMALL_T = 1024, CLIP_SMALL_CHUNKS = 32;
+template <bool MAX>
+__global__ __launch_bounds__(CLIP_SMALL_T) void norm_clip_kernel(const ClipChunk* __restrict__ chunks, int n_chunks, int writes,
+                                                                 double max_norm, double grad_scale, double* __restrict__ stats) {
+  __shared__ double red[CLIP_SMALL_T / 64];
+  const unsigned team = threadIdx.x / CLIP_T, t = threadIdx.x % CLIP_T;
+  ClipAcc acc;
+  for (int c = team; c < n_chunks; c += CLIP_SMALL_T / CLIP_T) norm_any<MAX>(chunks[c], t, acc);
+  const double raw = block_combine<MAX, CLIP_SMALL_T>(MAX ? (double)__uint_as_float(acc.mx) : acc.sum, red);
+  const float k = clip_factor<MAX>(raw, max_norm, grad_scale, stats, threadIdx.x == 0);
+  if (writes)
+    for (int c = team; c < n_chunks; c += CLIP_SMALL_T / CLIP_T) scale_any(chunks[c], t, k);
 }
 
 struct ClipPlan {
@@ -254,6 +400,13 @@ int jirf_train_grad_clip_run(const void* plan, int norm_kind, double max_norm, d
     hipStream_t s = static_cast<hipStream_t>(stream);
     const ClipChunk* ck = static_cast<const ClipChunk*>(pl->chunks.p);
     const bool mx = norm_kind == JIRF_NORM_MAX;
+    if (pl->n_chunks <= CLIP_SMALL_CHUNKS) {
+      Scope sc("train_grad_norm_clip", 3.0 * pl->total, pl->bytes_read + pl->bytes_written, s);
+      hipLaunchKernelGGL(mx ? norm_clip_kernel<true> : norm_clip_kernel<false>, dim3(1), dim3(CLIP_SMALL_T), 0, s, ck, pl->n_chunks,
+                         pl->writes ? 1 : 0, max_norm, grad_scale, stats);
+      JIRF_HIP_CHECK(hipGetLastError());
+      return JIRF_OK;
+    }
     {
       Scope sc("train_grad_norm", 2.0 * pl->total, pl->bytes_read, s);
       hipLaunchKernelGGL(mx ? norm_kernel<true> : norm_kernel<false>, dim3(pl->blocks), dim3(CLIP_T), 0, s, ck, pl->n_chunks, work);

@@ -1,0 +1,948 @@
+// Kernels of the residual join with its norms (formulas in residual_norm.hip), as templates over the activation type:
+// residual_norm_{f32,bf16,f16}.hip instantiate them, residual_norm.hip chooses among them.
+#pragma once
+
+#include "runtime.h"
+
+namespace jirf {
+
+struct RnArgs {
+  // activations, element (b, c, p) at ptr + b * bs + c * cs + p * ps
+  const void *x, *f, *dy, *dn, *y_in;
+  void *y, *n, *dx, *df;
+  long x_bs, f_bs, dy_bs, dn_bs, yi_bs, y_bs, n_bs, dx_bs, df_bs;
+  long cs, ps;
+  const float *post_w, *post_b, *gate, *scale, *pre_w, *pre_b;
+  const float* stats_in;   // [4][B][P]
+  float* stats;            // [4][B][P] or null
+  float* rowsum;           // backward of the sweep form: [2][B][P], the two row means of the pre norm's gradient
+  float* part;             // backward: [4][part_rows][C] partial sums, RN_Q_*
+  float* part_gate;        // backward, gate kind 2 and S > 1: [B][S][C]
+  float* dgate;            // backward, gate kind 2 and S == 1: written directly
+  long part_rows;
+  int post, pre, gate_kind, accumulate;
+  float eps;
+  int B, C, P;
+  // Workers: S per image, each a run of `per` tiles (ipw == 1), or one per ipw images (S == 1).
+  int S, ipw, per, tiles;
+};
+// The branch's parameter gradients come from two sums per channel, G1 = sum s dyt vh and G0 = sum s dyt (vh = the
+// normalised f, or f): dpost_w = gate G1, dpost_b = gate G0, dgate = post_w G1 + post_b G0 (or G1 without a norm).
+// With a gate per image the factors belong inside the sum over the images: then the sums are dpost_w and dpost_b.
+enum { RN_Q_G1 = 0, RN_Q_G0 = 1, RN_Q_PRE_W = 2, RN_Q_PRE_B = 3, RN_Q_N = 4 };
+
+// Which kernel serves a call.  lanes: tokens - threads per token (8..64, several tokens per wave) or 0 (the whole
+// workgroup); planar - pixel lanes; -1: the sweep form.
+struct RnForm {
+  bool tok;
+  int lanes, nv, threads;
+  unsigned blocks;
+};
+enum { RN_BWD_STREAM = 0, RN_BWD_BRANCH = 1, RN_BWD_IMAGE_GATE = 2 };
+
+template <typename T> void rn_launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s);
+template <typename T> void rn_launch_bwd(const RnArgs& a, const RnForm& f, int mode, bool params, hipStream_t s);
+
+}  // namespace jirf
+
+#ifdef JIRF_RN_KERNELS
+namespace jirf {
+namespace {
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ __forceinline__ float ld(const float* p) { return *p; }
+  static __device__ __forceinline__ void st(float* p, float v) { *p = v; }
+};
+template <> struct Elem<__bf16> {
+  static __device__ __forceinline__ float ld(const __bf16* p) { return (float)*p; }
+  static __device__ __forceinline__ void st(__bf16* p, float v) { *p = (__bf16)v; }
+};
+template <> struct Elem<_Float16> {
+  static __device__ __forceinline__ float ld(const _Float16* p) { return (float)*p; }
+  static __device__ __forceinline__ void st(_Float16* p, float v) { *p = (_Float16)v; }
+};
+
+// VEC consecutive elements as loaded, read and written at the alignment of one element (rows of odd length, channel slices:
+// the memory instructions take any 2- or 4-byte address).
+template <typename T, int VEC> struct Pack {
+  typedef T V __attribute__((ext_vector_type(VEC)));
+  typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+  V v;
+  // n < VEC: only the first n exist
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= VEC) {
+      v = *reinterpret_cast<const VU*>(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = i < n ? p[i] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, int n, const float* f) {
+  typedef T V __attribute__((ext_vector_type(VEC)));
+  typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+  V v;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = (T)f[i];
+  if (n >= VEC) {
+    *reinterpret_cast<VU*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i < n) p[i] = v[i];
+  }
+}
+
+constexpr int RN_T = 512;         // most threads of a workgroup in the register form (256 registers each)
+constexpr int RN_LANE_T = 256;    // threads of a workgroup whose waves hold several tokens each
+
+// ---- a tile in registers ------------------------------------------------------------------------------------------------
+// A worker owns a run of tiles; every thread holds NV vectors of VEC elements of each operand of a tile, so an operand is
+// read once.  tokens: a tile is one token, a vector VEC consecutive channels, and the token's threads are L lanes of a
+// wave (a worker per lane group) or the workgroup (L == 0).  planar: a tile is L * VEC pixels of all channels, a vector VEC
+// consecutive pixels of one channel; L lanes run along the pixels, the other threads along the channels.
+template <typename T, bool TOK, int L, int NV, int VEC>
+struct Tile {
+  static constexpr int NS = TOK ? 1 : VEC;       // statistics per thread: its token's, or one per pixel of its vector
+  static constexpr int NP = TOK ? VEC : 1;       // parameters per vector
+  typedef Pack<T, VEC> Vec;
+  const RnArgs& a;
+  float* red;                                    // LDS of two reductions
+  int buf;
+  int ch, nch, pl;                               // position among the token's threads, their number, pixel lane
+  int cnt[NV];                                   // tokens: channels of each vector that exist; planar: 0 or VEC
+  long off[NV];                                  // offset of each vector's first element from the tile's first
+
+  static constexpr int RED = TOK ? (L ? 1 : 2 * 8 * 2) : 2 * 8 * L * 2 * VEC;
+
+  __device__ __forceinline__ Tile(const RnArgs& args, float* lds) : a(args), red(lds), buf(0) {
+    const int tid = threadIdx.x;
+    if (TOK) {
+      ch = L ? tid & (L - 1) : tid;
+      nch = L ? L : blockDim.x;
+      pl = 0;
+    } else {
+      pl = tid & (L - 1);
+      ch = tid / L;
+      nch = blockDim.x / L;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = channel(j);
+      if (TOK) {
+        cnt[j] = max(0, min(VEC, a.C - c));
+        off[j] = c;
+      } else {
+        cnt[j] = c < a.C ? VEC : 0;
+        off[j] = (long)c * a.P + pl * VEC;
+      }
+    }
+  }
+  __device__ __forceinline__ int channel(int j) const { return TOK ? (j * nch + ch) * VEC : j * nch + ch; }
+  // elements of vector j inside tile t
+  __device__ __forceinline__ int count(int j, int t) const {
+    if (TOK) return cnt[j];
+    const long left = (long)a.P - ((long)t * L + pl) * VEC;
+    return cnt[j] ? (int)min(left, (long)VEC) : 0;
+  }
+  __device__ __forceinline__ bool exists(int j, int v) const { return TOK ? v < cnt[j] : cnt[j] > 0; }
+  __device__ __forceinline__ long origin(int b, long bs, int t) const {
+    return b * bs + (TOK ? (long)t * a.C : (long)t * (L * VEC));
+  }
+  __device__ __forceinline__ void load(const T* base, int t, Vec (&r)[NV]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int n = count(j, t);
+      if (n > 0) r[j].load(base + off[j], n);
+      else r[j].v = typename Vec::V(0);
+    }
+  }
+  __device__ __forceinline__ void store(T* base, int t, const float (&f)[NV][VEC]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int n = count(j, t);
+      if (n > 0) store_vec<T, VEC>(base + off[j], n, f[j]);
+    }
+  }
+  // a [C] array in the thread's channels; `none` where there is no channel or no array
+  __device__ __forceinline__ void params(const float* p, float none, float (&r)[NV][NP]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int v = 0; v < NP; ++v) r[j][v] = p && exists(j, v) ? p[channel(j) + v] : none;
+  }
+  // Sums v[0..N) over the threads of the token.  Lanes first, then the waves in order through LDS; two buffers in turn, so
+  // one barrier per reduction is enough.
+  template <int N>
+  __device__ __forceinline__ void reduce(float (&v)[N]) {
+    if (TOK && L) {
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+      return;
+    }
+#pragma unroll
+    for (int o = 32; o >= (TOK ? 1 : L); o >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if (waves == 1) return;
+    constexpr int W = TOK ? 1 : L;
+    float* r = red + buf * (RED / 2);
+    buf ^= 1;
+    if (lane < W)
+#pragma unroll
+      for (int i = 0; i < N; ++i) r[(wave * W + lane) * N + i] = v[i];
+    __syncthreads();
+    const int at = TOK ? 0 : pl;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = r[at * N + i];
+    for (int w = 1; w < waves; ++w)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += r[(w * W + at) * N + i];
+  }
+  // mean (0 for the root mean square) and reciprocal deviation, in two passes over the registers
+  __device__ __forceinline__ void statistics(const float (&v)[NV][VEC], int kind, float (&mu)[NS], float (&rs)[NS]) {
+    const float inv = 1.0f / (float)a.C;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) mu[s] = 0.f;
+    if (kind != 3) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) mu[TOK ? 0 : i] += v[j][i];       // (absent elements are 0)
+      reduce<NS>(mu);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) mu[s] *= inv;
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) rs[s] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float d = exists(j, i) ? v[j][i] - mu[TOK ? 0 : i] : 0.f;
+        rs[TOK ? 0 : i] = fmaf(d, d, rs[TOK ? 0 : i]);
+      }
+    reduce<NS>(rs);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) rs[s] = 1.0f / sqrtf(fmaf(rs[s], inv, a.eps));
+  }
+  // images [b0, b1) and tiles [t0, t1) of worker w
+  __device__ __forceinline__ void range(long w, int& b0, int& b1, int& t0, int& t1, int& slab) const {
+    if (a.S > 1) {
+      b0 = (int)min(w / a.S, (long)a.B);
+      b1 = min(b0 + 1, a.B);
+      slab = (int)(w % a.S);
+      t0 = min(a.tiles, slab * a.per);
+      t1 = min(a.tiles, t0 + a.per);
+    } else {
+      b0 = (int)min(w * a.ipw, (long)a.B);
+      b1 = (int)min(w * a.ipw + a.ipw, (long)a.B);
+      slab = 0;
+      t0 = 0;
+      t1 = a.tiles;
+    }
+  }
+  __device__ __forceinline__ long worker() const {
+    if (TOK && L) return (long)blockIdx.x * (blockDim.x / L) + threadIdx.x / L;
+    return blockIdx.x;
+  }
+};
+
+// Forward.  Reads x and f once and writes y and n once; the next tile's loads are issued before this tile's reductions.
+// The branch's factors are folded: u = vh (gate w) + gate b.
+template <typename T, bool TOK, int L, int NV, int VEC>
+__global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
+  typedef Tile<T, TOK, L, NV, VEC> Ti;
+  typedef typename Ti::Vec Vec;
+  constexpr int NS = Ti::NS, NP = Ti::NP;
+  __shared__ float lds[Ti::RED];
+  Ti ti(a, lds);
+  int b0, b1, t0, t1, slab;
+  ti.range(ti.worker(), b0, b1, t0, t1, slab);
+  if (b0 >= b1 || t0 >= t1) return;           // (uniform over the threads of a worker, and a worker's barriers are its own)
+  float pw[NV][NP], pb[NV][NP], gw[NV][NP], gb[NV][NP];
+  ti.params(a.pre ? a.pre_w : nullptr, 0.f, pw);
+  ti.params(a.pre == 1 ? a.pre_b : nullptr, 0.f, pb);
+  const T* xp = static_cast<const T*>(a.x);
+  const T* fp = static_cast<const T*>(a.f);
+  Vec xn[NV], fn[NV];
+  ti.load(fp + ti.origin(b0, a.f_bs, t0), t0, fn);
+  ti.load(xp + ti.origin(b0, a.x_bs, t0), t0, xn);
+  int gate_of = -1;
+  for (int b = b0; b < b1; ++b) {
+    if (gate_of < 0 || a.gate_kind == 2) {
+      gate_of = b;
+      ti.params(a.post ? a.post_w : nullptr, 1.f, gw);
+      ti.params(a.post == 1 ? a.post_b : nullptr, 0.f, gb);
+      if (a.gate_kind) {
+        float g[NV][NP];
+        ti.params(a.gate + (a.gate_kind == 2 ? (long)b * a.C : 0), 0.f, g);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            gw[j][i] *= g[j][i];
+            gb[j][i] *= g[j][i];
+          }
+      }
+    }
+    const float s = a.scale ? a.scale[b] : 1.0f;
+    for (int t = t0; t < t1; ++t) {
+      Vec xv[NV], fv[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        xv[j] = xn[j];
+        fv[j] = fn[j];
+      }
+      const int bn = t + 1 < t1 ? b : b + 1, tn = t + 1 < t1 ? t + 1 : t0;
+      if (bn < b1) {
+        ti.load(fp + ti.origin(bn, a.f_bs, tn), tn, fn);
+        ti.load(xp + ti.origin(bn, a.x_bs, tn), tn, xn);
+      }
+      float v[NV][VEC], mu0[NS], rs0[NS], mu1[NS], rs1[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) mu0[i] = rs0[i] = mu1[i] = rs1[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j][i] = fv[j].at(i);
+      if (a.post) {
+        ti.statistics(v, a.post, mu0, rs0);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[j][i] = (a.post == 1 ? v[j][i] - mu0[TOK ? 0 : i] : v[j][i]) * rs0[TOK ? 0 : i];
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          v[j][i] = ti.exists(j, i) ? fmaf(s, fmaf(v[j][i], gw[j][TOK ? i : 0], gb[j][TOK ? i : 0]), xv[j].at(i)) : 0.f;
+      ti.store(static_cast<T*>(a.y) + ti.origin(b, a.y_bs, t), t, v);
+      if (a.pre) {
+        ti.statistics(v, a.pre, mu1, rs1);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            v[j][i] = fmaf((a.pre == 1 ? v[j][i] - mu1[TOK ? 0 : i] : v[j][i]) * rs1[TOK ? 0 : i], pw[j][TOK ? i : 0], pb[j][TOK ? i : 0]);
+        ti.store(static_cast<T*>(a.n) + ti.origin(b, a.n_bs, t), t, v);
+      }
+      if (a.stats && ti.ch == 0) {
+        const long bp = (long)a.B * a.P;
+        const long p0 = TOK ? t : ((long)t * L + ti.pl) * VEC;
+        float* st = a.stats + (long)b * a.P + p0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+          if (p0 + i < a.P) {
+            st[i] = mu0[i];
+            st[bp + i] = rs0[i];
+            st[2 * bp + i] = mu1[i];
+            st[3 * bp + i] = rs1[i];
+          }
+      }
+    }
+  }
+}
+
+// Backward.  Every operand once; the parameter gradients accumulate in the registers of the threads that hold the
+// channel, over all of the worker's tiles, and are added up across lanes and waves once, at the end.
+template <typename T, bool TOK, int L, int NV, int VEC, int MODE>
+__global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
+  typedef Tile<T, TOK, L, NV, VEC> Ti;
+  typedef typename Ti::Vec Vec;
+  constexpr int NS = Ti::NS, NP = Ti::NP;
+  constexpr bool BR = MODE != RN_BWD_STREAM, IG = MODE == RN_BWD_IMAGE_GATE;
+  constexpr int EW = NV * NP;                                  // channels of a thread
+  __shared__ float lds[Ti::RED];
+  __shared__ float wsum[TOK && L ? RN_LANE_T / 64 * L * EW : 1];
+  Ti ti(a, lds);
+  int b0, b1, t0, t1, slab;
+  ti.range(ti.worker(), b0, b1, t0, t1, slab);
+  if (t0 >= t1) b1 = b0;                                       // nothing to do, but its partial sums are written (zeros)
+  float acc[RN_Q_N][NV][NP], img[2][NV][NP];                   // img: G1, G0 of the current image
+#pragma unroll
+  for (int q = 0; q < RN_Q_N; ++q)
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < NP; ++i) acc[q][j][i] = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) img[0][j][i] = img[1][j][i] = 0.f;
+  float pw[NV][NP], gw[NV][NP];
+  ti.params(a.pre ? a.pre_w : nullptr, 0.f, pw);
+  const T* dyp = static_cast<const T*>(a.dy);
+  const T* dnp = static_cast<const T*>(a.dn);
+  const T* yp = static_cast<const T*>(a.y_in);
+  const T* fp = static_cast<const T*>(a.f);
+  const float inv = 1.0f / (float)a.C;
+  const long bp = (long)a.B * a.P;
+  Vec dyn[NV], dnn[NV], yn[NV], fn[NV];
+  auto fetch = [&](int b, int t) {
+    if (a.dy) ti.load(dyp + ti.origin(b, a.dy_bs, t), t, dyn);
+    if (a.pre) {
+      ti.load(dnp + ti.origin(b, a.dn_bs, t), t, dnn);
+      ti.load(yp + ti.origin(b, a.yi_bs, t), t, yn);
+    }
+    if (BR) ti.load(fp + ti.origin(b, a.f_bs, t), t, fn);
+  };
+#pragma unroll
+  for (int j = 0; j < NV; ++j) dyn[j].v = dnn[j].v = yn[j].v = fn[j].v = typename Vec::V(0);
+  if (b0 < b1) fetch(b0, t0);
+  bool have_gw = false;
+  for (int b = b0; b < b1; ++b) {
+    if (BR && (!have_gw || IG)) {
+      have_gw = true;
+      ti.params(a.post ? a.post_w : nullptr, 1.f, gw);
+      if (a.gate_kind) {
+        float g[NV][NP];
+        ti.params(a.gate + (IG ? (long)b * a.C : 0), 0.f, g);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < NP; ++i) gw[j][i] *= g[j][i];
+      }
+    }
+    const float s = a.scale ? a.scale[b] : 1.0f;
+    for (int t = t0; t < t1; ++t) {
+      Vec dy[NV], dn[NV], yv[NV], fv[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        dy[j] = dyn[j];
+        dn[j] = dnn[j];
+        yv[j] = yn[j];
+        fv[j] = fn[j];
+      }
+      const int bn = t + 1 < t1 ? b : b + 1, tn = t + 1 < t1 ? t + 1 : t0;
+      if (bn < b1) fetch(bn, tn);
+      // statistics of the token(s); a pixel past the end has deviation 0 and adds nothing
+      float mu0[NS], rs0[NS], mu1[NS], rs1[NS];
+      {
+        const long p0 = TOK ? t : ((long)t * L + ti.pl) * VEC;
+        const float* st = a.stats_in + (long)b * a.P + p0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          const bool on = TOK || p0 + i < a.P;
+          mu0[i] = BR && a.post && on ? st[i] : 0.f;
+          rs0[i] = BR && a.post ? (on ? st[bp + i] : 0.f) : 1.f;
+          mu1[i] = a.pre && on ? st[2 * bp + i] : 0.f;
+          rs1[i] = a.pre && on ? st[3 * bp + i] : 0.f;
+        }
+      }
+      float d[NV][VEC];                                        // dyt
+      if (a.pre) {
+        float m[2 * NS];
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i) m[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const int q = TOK ? 0 : i, c = TOK ? i : 0;
+            const float o = dn[j].at(i), g = o * pw[j][c];
+            const float vh = (a.pre == 1 ? yv[j].at(i) - mu1[q] : yv[j].at(i)) * rs1[q];
+            m[q] += g;
+            m[NS + q] = fmaf(g, vh, m[NS + q]);
+            acc[RN_Q_PRE_W][j][c] = fmaf(o, vh, acc[RN_Q_PRE_W][j][c]);
+            acc[RN_Q_PRE_B][j][c] += o;
+          }
+        ti.template reduce<2 * NS>(m);
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          m[i] = a.pre == 1 ? m[i] * inv : 0.f;
+          m[NS + i] *= inv;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const int q = TOK ? 0 : i, c = TOK ? i : 0;
+            const float cent = (yv[j].at(i) - mu1[q]) * rs1[q];
+            d[j][i] = fmaf(rs1[q], dn[j].at(i) * pw[j][c] - m[q] - cent * m[NS + q], dy[j].at(i));
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) d[j][i] = dy[j].at(i);
+      }
+      ti.store(static_cast<T*>(a.dx) + ti.origin(b, a.dx_bs, t), t, d);
+      if (!BR) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) d[j][i] *= s;
+      } else {
+        float m[2 * NS];
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i) m[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const int q = TOK ? 0 : i, c = TOK ? i : 0;
+            const float sd = ti.exists(j, i) ? d[j][i] * s : 0.f;
+            const float vh = (a.post == 1 ? fv[j].at(i) - mu0[q] : fv[j].at(i)) * rs0[q];
+            img[0][j][c] = fmaf(sd, vh, img[0][j][c]);
+            // (a pixel past the end has dyt = 0: its dy is 0 and its deviation is 0)
+            img[1][j][c] += sd;
+            d[j][i] = sd * gw[j][c];
+            m[q] += d[j][i];
+            m[NS + q] = fmaf(d[j][i], vh, m[NS + q]);
+          }
+        if (a.post) {
+          ti.template reduce<2 * NS>(m);
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            m[i] = a.post == 1 ? m[i] * inv : 0.f;
+            m[NS + i] *= inv;
+          }
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const int q = TOK ? 0 : i;
+              d[j][i] = rs0[q] * (d[j][i] - m[q] - (fv[j].at(i) - mu0[q]) * rs0[q] * m[NS + q]);
+            }
+        }
+      }
+      ti.store(static_cast<T*>(a.df) + ti.origin(b, a.df_bs, t), t, d);
+    }
+    if (IG) {
+      // the image is done: its gate's gradient, and its share of the norm's parameters
+      float w0[NV][NP], bb[NV][NP], g[NV][NP];
+      ti.params(a.post ? a.post_w : nullptr, 1.f, w0);
+      ti.params(a.post == 1 ? a.post_b : nullptr, 0.f, bb);
+      ti.params(a.gate + (long)b * a.C, 0.f, g);
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          float g1 = img[0][j][i], g0 = img[1][j][i];
+          if (!TOK) {
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) {
+              g1 += __shfl_xor(g1, o);
+              g0 += __shfl_xor(g0, o);
+            }
+          }
+          acc[RN_Q_G1][j][i] = fmaf(img[0][j][i], g[j][i], acc[RN_Q_G1][j][i]);
+          acc[RN_Q_G0][j][i] = fmaf(img[1][j][i], g[j][i], acc[RN_Q_G0][j][i]);
+          img[0][j][i] = img[1][j][i] = 0.f;
+          const float dg = fmaf(g1, w0[j][i], g0 * bb[j][i]);
+          if (ti.exists(j, i) && (TOK || ti.pl == 0)) {
+            const int c = ti.channel(j) + i;
+            if (a.S > 1) {
+              if (a.part_gate) a.part_gate[((long)b * a.S + slab) * a.C + c] = dg;
+            } else if (a.dgate) {
+              a.dgate[(long)b * a.C + c] = a.accumulate ? a.dgate[(long)b * a.C + c] + dg : dg;
+            }
+          }
+        }
+    }
+  }
+  if (IG && a.S > 1 && a.part_gate && b0 >= b1) {
+    // a worker without tiles still owns a row of the gate's partial sums
+    const int b = (int)(ti.worker() / a.S);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        if (b < a.B && ti.exists(j, i) && (TOK || ti.pl == 0)) a.part_gate[((long)b * a.S + slab) * a.C + ti.channel(j) + i] = 0.f;
+  }
+  if (!a.part) return;
+  // one row of partial sums per workgroup
+#pragma unroll
+  for (int q = 0; q < RN_Q_N; ++q) {
+    if (!BR && q < RN_Q_PRE_W) continue;
+    if (q >= RN_Q_PRE_W && !a.pre) continue;
+    float* out = a.part + ((long)q * a.part_rows + blockIdx.x) * a.C;
+    if (TOK && L) {
+      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          float v = BR && !IG && q < RN_Q_PRE_W ? img[q][j][i] : acc[q][j][i];
+#pragma unroll
+          for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o);
+          if (lane < L) wsum[(wave * L + lane) * EW + j * NP + i] = v;
+        }
+      __syncthreads();
+      for (int k = threadIdx.x; k < L * EW; k += blockDim.x) {
+        const int l = k / EW, e = k % EW, c = ((e / NP) * L + l) * VEC + e % NP;
+        float v = 0.f;
+        for (int w = 0; w < waves; ++w) v += wsum[(w * L + l) * EW + e];
+        if (c < a.C) out[c] = v;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+          float v = BR && !IG && q < RN_Q_PRE_W ? img[q][j][i] : acc[q][j][i];
+          if (!TOK) {
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o);
+          }
+          if (ti.exists(j, i) && (TOK || ti.pl == 0)) out[ti.channel(j) + i] = v;
+        }
+    }
+  }
+}
+
+// ---- any number of channels -------------------------------------------------------------------------------------------
+// One workgroup per token (tokens layout, 256 threads along the channels) or per 64 pixels (planar, four waves along
+// the channels); nothing is kept between the passes over the channels, each reads its operands again.
+template <bool TOK>
+struct Sweep {
+  float* red;
+  // sum over the threads that share a token
+  __device__ __forceinline__ float sum(float v) const {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    if (TOK) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+      if ((tid & 63) == 0) red[tid >> 6] = v;
+      __syncthreads();
+      return (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    red[tid] = v;
+    __syncthreads();
+    const int l = tid & 63;
+    return (red[l] + red[64 + l]) + (red[128 + l] + red[192 + l]);
+  }
+};
+
+template <typename T, bool TOK>
+__global__ __launch_bounds__(256) void rn_fwd_sweep(const RnArgs a) {
+  __shared__ float red[256];
+  const Sweep<TOK> sw{red};
+  const int tid = threadIdx.x;
+  const long tiles = TOK ? a.P : (a.P + 63) / 64;
+  const int c0 = TOK ? tid : tid >> 6, dc = TOK ? 256 : 4;
+  const float inv = 1.0f / (float)a.C;
+  for (long t = blockIdx.x; t < tiles * a.B; t += gridDim.x) {
+    const long b = t / tiles, pt = t % tiles;
+    const long p = TOK ? pt : pt * 64 + (tid & 63);
+    const bool on = p < a.P;
+    const long o = (on ? p : 0) * a.ps;
+    const T* x = static_cast<const T*>(a.x) + b * a.x_bs + o;
+    const T* f = static_cast<const T*>(a.f) + b * a.f_bs + o;
+    T* y = static_cast<T*>(a.y) + b * a.y_bs + o;
+    T* n = static_cast<T*>(a.n) + (a.pre ? b * a.n_bs + o : 0);
+    const float s = a.scale ? a.scale[b] : 1.0f;
+    const float* gate = a.gate_kind == 2 ? a.gate + b * a.C : a.gate;
+    float mu0 = 0.f, rs0 = 0.f, mu1 = 0.f, rs1 = 0.f;
+    if (a.post) {
+      float q = 0.f;
+      if (a.post != 3) {
+        for (int c = c0; c < a.C; c += dc) q += Elem<T>::ld(f + c * a.cs);
+        mu0 = sw.sum(q) * inv;
+      }
+      q = 0.f;
+      for (int c = c0; c < a.C; c += dc) {
+        const float d = Elem<T>::ld(f + c * a.cs) - mu0;
+        q = fmaf(d, d, q);
+      }
+      rs0 = 1.0f / sqrtf(sw.sum(q) * inv + a.eps);
+    }
+    auto join = [&](int c) {
+      float u = Elem<T>::ld(f + c * a.cs);
+      if (a.post) {
+        u = (a.post == 1 ? u - mu0 : u) * rs0 * a.post_w[c];
+        if (a.post == 1 && a.post_b) u += a.post_b[c];
+      }
+      return fmaf(a.gate_kind ? s * gate[c] : s, u, Elem<T>::ld(x + c * a.cs));
+    };
+    if (a.pre) {
+      float q = 0.f;
+      if (a.pre != 3) {
+        for (int c = c0; c < a.C; c += dc) q += join(c);
+        mu1 = sw.sum(q) * inv;
+      }
+      q = 0.f;
+      for (int c = c0; c < a.C; c += dc) {
+        const float d = join(c) - mu1;
+        q = fmaf(d, d, q);
+      }
+      rs1 = 1.0f / sqrtf(sw.sum(q) * inv + a.eps);
+    }
+    if (on) {
+      for (int c = c0; c < a.C; c += dc) {      // y may be x and n may be f: a thread reads both before it writes
+        const float v = join(c);
+        Elem<T>::st(y + c * a.cs, v);
+        if (a.pre) {
+          float r = (a.pre == 1 ? v - mu1 : v) * rs1 * a.pre_w[c];
+          if (a.pre == 1 && a.pre_b) r += a.pre_b[c];
+          Elem<T>::st(n + c * a.cs, r);
+        }
+      }
+      if (a.stats && c0 == 0) {
+        const long bp = (long)a.B * a.P, at = b * a.P + p;
+        a.stats[at] = mu0;
+        a.stats[bp + at] = rs0;
+        a.stats[2 * bp + at] = mu1;
+        a.stats[3 * bp + at] = rs1;
+      }
+    }
+  }
+}
+
+// What the backward's element formulas need of one token.
+struct RowBwd {
+  float mu0, rs0, mu1, rs1, m1, m2, s;
+};
+
+// dyt of one element: dy + rs (g - [kind 1] mean g - c mean(g vh))
+__device__ __forceinline__ float rn_dyt(const RnArgs& a, const RowBwd& r, float dy, float dn, float y, float w) {
+  if (!a.pre) return dy;
+  return dy + r.rs1 * (dn * w - r.m1 - (y - r.mu1) * r.rs1 * r.m2);
+}
+
+template <typename T, bool TOK>
+__global__ __launch_bounds__(256) void rn_bwd_sweep(const RnArgs a) {
+  __shared__ float red[256];
+  const Sweep<TOK> sw{red};
+  const int tid = threadIdx.x;
+  const long tiles = TOK ? a.P : (a.P + 63) / 64;
+  const int c0 = TOK ? tid : tid >> 6, dc = TOK ? 256 : 4;
+  const float inv = 1.0f / (float)a.C;
+  const long bp = (long)a.B * a.P;
+  for (long t = blockIdx.x; t < tiles * a.B; t += gridDim.x) {
+    const long b = t / tiles, pt = t % tiles;
+    const long p = TOK ? pt : pt * 64 + (tid & 63);
+    const bool on = p < a.P;
+    const long o = (on ? p : 0) * a.ps, at = b * a.P + (on ? p : 0);
+    const T* dy = a.dy ? static_cast<const T*>(a.dy) + b * a.dy_bs + o : nullptr;
+    const T* dn = a.pre ? static_cast<const T*>(a.dn) + b * a.dn_bs + o : nullptr;
+    const T* y = a.pre ? static_cast<const T*>(a.y_in) + b * a.yi_bs + o : nullptr;
+    const T* f = a.post ? static_cast<const T*>(a.f) + b * a.f_bs + o : nullptr;
+    T* dx = static_cast<T*>(a.dx) + b * a.dx_bs + o;
+    T* df = static_cast<T*>(a.df) + b * a.df_bs + o;
+    const float* gate = a.gate_kind == 2 ? a.gate + b * a.C : a.gate;
+    RowBwd r{};
+    r.s = a.scale ? a.scale[b] : 1.0f;
+    if (a.post) {
+      r.mu0 = a.stats_in[at];
+      r.rs0 = a.stats_in[bp + at];
+    }
+    if (a.pre) {
+      r.mu1 = a.stats_in[2 * bp + at];
+      r.rs1 = a.stats_in[3 * bp + at];
+      const float m = a.pre == 1 ? r.mu1 : 0.f;
+      float s1 = 0.f, s2 = 0.f;
+      for (int c = c0; c < a.C; c += dc) {
+        const float g = Elem<T>::ld(dn + c * a.cs) * a.pre_w[c];
+        s1 += g;
+        s2 = fmaf(g, (Elem<T>::ld(y + c * a.cs) - m) * r.rs1, s2);
+      }
+      r.m1 = a.pre == 1 ? sw.sum(s1) * inv : 0.f;
+      r.m2 = sw.sum(s2) * inv;
+      if (on && c0 == 0) {
+        a.rowsum[at] = r.m1;
+        a.rowsum[bp + at] = r.m2;
+      }
+    }
+    auto dyt = [&](int c) {
+      return rn_dyt(a, r, dy ? Elem<T>::ld(dy + c * a.cs) : 0.f, a.pre ? Elem<T>::ld(dn + c * a.cs) : 0.f,
+                    a.pre ? Elem<T>::ld(y + c * a.cs) : 0.f, a.pre ? a.pre_w[c] : 0.f);
+    };
+    float t1 = 0.f, t2 = 0.f;
+    if (a.post) {
+      const float m = a.post == 1 ? r.mu0 : 0.f;
+      for (int c = c0; c < a.C; c += dc) {
+        const float g = dyt(c) * (a.gate_kind ? r.s * gate[c] : r.s) * a.post_w[c];
+        t1 += g;
+        t2 = fmaf(g, (Elem<T>::ld(f + c * a.cs) - m) * r.rs0, t2);
+      }
+      t1 = a.post == 1 ? sw.sum(t1) * inv : 0.f;
+      t2 = sw.sum(t2) * inv;
+    }
+    if (on)
+      for (int c = c0; c < a.C; c += dc) {
+        const float d = dyt(c);
+        float du = d * (a.gate_kind ? r.s * gate[c] : r.s);
+        if (a.post) du = r.rs0 * (du * a.post_w[c] - t1 - (Elem<T>::ld(f + c * a.cs) - r.mu0) * r.rs0 * t2);
+        Elem<T>::st(dx + c * a.cs, d);
+        Elem<T>::st(df + c * a.cs, du);
+      }
+  }
+}
+
+// The parameter gradients of the sweep form: one pass more over the operands, a workgroup per 64 channels and worker
+// (tokens: lanes along the channels, waves along the rows; planar: a wave per channel, lanes along the pixels).
+template <typename T, bool TOK>
+__global__ __launch_bounds__(256) void rn_bwd_params_sweep(const RnArgs a) {
+  __shared__ float red[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int worker = blockIdx.y;
+  const int b0 = a.S > 1 ? worker / a.S : worker * a.ipw, b1 = min(a.B, a.S > 1 ? b0 + 1 : b0 + a.ipw);
+  const int slab = a.S > 1 ? worker % a.S : 0;
+  const long p0 = min((long)a.P, (long)slab * a.per * 64), p1 = a.S > 1 ? min((long)a.P, p0 + (long)a.per * 64) : a.P;
+  const long bp = (long)a.B * a.P;
+  const int c = blockIdx.x * (TOK ? 64 : 4) + (TOK ? lane : wave);
+  const bool on = c < a.C;
+  const int cc = on ? c : 0;
+  float acc[RN_Q_N] = {0.f, 0.f, 0.f, 0.f};
+  // per-channel sums across the threads that share the channel
+  auto total = [&](float v) {
+    if (!TOK) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+      return v;
+    }
+    __syncthreads();
+    red[tid] = v;
+    __syncthreads();
+    return (red[lane] + red[64 + lane]) + (red[128 + lane] + red[192 + lane]);
+  };
+  const bool writer = on && (TOK ? wave == 0 : lane == 0);
+  const bool branch = a.post || a.gate_kind;
+  for (int b = b0; b < b1; ++b) {
+    const float s = a.scale ? a.scale[b] : 1.0f;
+    const float w1 = a.pre ? a.pre_w[cc] : 0.f;
+    float g1 = 0.f, g0 = 0.f;
+    for (long p = p0 + (TOK ? wave : lane); p < p1; p += TOK ? 4 : 64) {
+      const long o = p * a.ps + cc * a.cs, at = (long)b * a.P + p;
+      RowBwd r{};
+      float dnv = 0.f, yv = 0.f;
+      if (a.pre) {
+        r.mu1 = a.stats_in[2 * bp + at];
+        r.rs1 = a.stats_in[3 * bp + at];
+        r.m1 = a.rowsum[at];
+        r.m2 = a.rowsum[bp + at];
+        dnv = Elem<T>::ld(static_cast<const T*>(a.dn) + b * a.dn_bs + o);
+        yv = Elem<T>::ld(static_cast<const T*>(a.y_in) + b * a.yi_bs + o);
+        acc[RN_Q_PRE_W] = fmaf(dnv, (a.pre == 1 ? yv - r.mu1 : yv) * r.rs1, acc[RN_Q_PRE_W]);
+        acc[RN_Q_PRE_B] += dnv;
+      }
+      if (!branch) continue;
+      const float d = rn_dyt(a, r, a.dy ? Elem<T>::ld(static_cast<const T*>(a.dy) + b * a.dy_bs + o) : 0.f, dnv, yv, w1) * s;
+      float u = Elem<T>::ld(static_cast<const T*>(a.f) + b * a.f_bs + o);
+      if (a.post) u = (a.post == 1 ? u - a.stats_in[at] : u) * a.stats_in[bp + at];
+      g1 = fmaf(d, u, g1);
+      g0 += d;
+    }
+    if (branch && a.gate_kind == 2) {
+      const float w0 = a.post ? a.post_w[cc] : 1.f, bb = a.post == 1 && a.post_b ? a.post_b[cc] : 0.f;
+      const float gt = a.gate[(long)b * a.C + cc];
+      const float dg = fmaf(total(g1), w0, total(g0) * bb);
+      if (writer) {
+        if (a.S > 1) {
+          if (a.part_gate) a.part_gate[((long)b * a.S + slab) * a.C + c] = dg;
+        } else if (a.dgate) {
+          a.dgate[(long)b * a.C + c] = a.accumulate ? a.dgate[(long)b * a.C + c] + dg : dg;
+        }
+      }
+      g1 *= gt;
+      g0 *= gt;
+    }
+    acc[RN_Q_G1] += g1;
+    acc[RN_Q_G0] += g0;
+  }
+#pragma unroll
+  for (int q = 0; q < RN_Q_N; ++q) {
+    const float v = total(acc[q]);
+    if (writer) a.part[((long)q * a.part_rows + worker) * a.C + c] = v;
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+// Vectors: 16 bytes of channels per thread in the token layout, four pixels in the planar one.
+template <typename T> constexpr int rn_vec(bool tok) { return tok ? 16 / (int)sizeof(T) : 4; }
+unsigned sweep_blocks(bool tok, int B, int P) {
+  const long tiles = (tok ? (long)P : ((long)P + 63) / 64) * B;
+  return (unsigned)std::min<long>(tiles, 1 << 16);
+}
+
+#define RN_FWD(TOK, L, NV)                                                                                                \
+  hipLaunchKernelGGL((rn_fwd_tile<T, TOK, L, NV, rn_vec<T>(TOK)>), dim3(f.blocks), dim3(f.threads), 0, s, a)
+template <typename T>
+void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
+  constexpr int E8 = 8 / rn_vec<T>(true);       // vectors for eight channels per thread
+  if (f.lanes < 0) {
+    if (f.tok) hipLaunchKernelGGL((rn_fwd_sweep<T, true>), dim3(sweep_blocks(true, a.B, a.P)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((rn_fwd_sweep<T, false>), dim3(sweep_blocks(false, a.B, a.P)), dim3(256), 0, s, a);
+  } else if (f.tok) {
+    switch (f.lanes) {
+      case 8: RN_FWD(true, 8, E8); break;
+      case 16: RN_FWD(true, 16, E8); break;
+      case 32: RN_FWD(true, 32, E8); break;
+      case 64: RN_FWD(true, 64, E8); break;
+      default:
+        if (f.nv == E8) RN_FWD(true, 0, E8);
+        else RN_FWD(true, 0, 2 * E8);
+    }
+  } else {
+    switch (f.lanes) {
+      case 2: RN_FWD(false, 2, 4); break;
+      case 4: RN_FWD(false, 4, 4); break;
+      case 8: RN_FWD(false, 8, 4); break;
+      case 16: RN_FWD(false, 16, 4); break;
+      default: RN_FWD(false, 32, 4);
+    }
+  }
+}
+#undef RN_FWD
+
+#define RN_BWD(TOK, L, NV)                                                                                                \
+  hipLaunchKernelGGL((rn_bwd_tile<T, TOK, L, NV, rn_vec<T>(TOK), MODE>), dim3(f.blocks), dim3(f.threads), 0, s, a)
+template <typename T, int MODE>
+void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
+  constexpr int E8 = 8 / rn_vec<T>(true);
+  if (f.tok) {
+    switch (f.lanes) {
+      case 8: RN_BWD(true, 8, E8); break;
+      case 16: RN_BWD(true, 16, E8); break;
+      case 32: RN_BWD(true, 32, E8); break;
+      case 64: RN_BWD(true, 64, E8); break;
+      default:
+        if (f.nv == E8) RN_BWD(true, 0, E8);
+        else RN_BWD(true, 0, 2 * E8);
+    }
+  } else {
+    switch (f.lanes) {
+      case 2: RN_BWD(false, 2, 4); break;
+      case 4: RN_BWD(false, 4, 4); break;
+      case 8: RN_BWD(false, 8, 4); break;
+      case 16: RN_BWD(false, 16, 4); break;
+      default: RN_BWD(false, 32, 4);
+    }
+  }
+}
+#undef RN_BWD
+template <typename T>
+void launch_bwd(const RnArgs& a, const RnForm& f, int mode, bool params, hipStream_t s) {
+  if (f.lanes < 0) {
+    const dim3 grid(sweep_blocks(f.tok, a.B, a.P));
+    const dim3 pgrid((unsigned)((a.C + (f.tok ? 63 : 3)) / (f.tok ? 64 : 4)), (unsigned)a.part_rows);
+    if (f.tok) {
+      hipLaunchKernelGGL((rn_bwd_sweep<T, true>), grid, dim3(256), 0, s, a);
+      if (params) hipLaunchKernelGGL((rn_bwd_params_sweep<T, true>), pgrid, dim3(256), 0, s, a);
+    } else {
+      hipLaunchKernelGGL((rn_bwd_sweep<T, false>), grid, dim3(256), 0, s, a);
+      if (params) hipLaunchKernelGGL((rn_bwd_params_sweep<T, false>), pgrid, dim3(256), 0, s, a);
+    }
+  } else if (mode == RN_BWD_STREAM) {
+    launch_bwd_tile<T, RN_BWD_STREAM>(a, f, s);
+  } else if (mode == RN_BWD_BRANCH) {
+    launch_bwd_tile<T, RN_BWD_BRANCH>(a, f, s);
+  } else {
+    launch_bwd_tile<T, RN_BWD_IMAGE_GATE>(a, f, s);
+  }
+}
+
+}  // namespace
+}  // namespace jirf
+#endif  // JIRF_RN_KERNELS

@@ -21,328 +21,10 @@
 #include <algorithm>
 #include <cmath>
 
-#include "runtime.h"
+#include "residual_norm.h"
 
 namespace jirf {
 namespace {
-
-template <typename T> struct Elem;
-template <> struct Elem<float> {
-  static __device__ __forceinline__ float ld(const float* p) { return *p; }
-  static __device__ __forceinline__ void st(float* p, float v) { *p = v; }
-};
-template <> struct Elem<__bf16> {
-  static __device__ __forceinline__ float ld(const __bf16* p) { return (float)*p; }
-  static __device__ __forceinline__ void st(__bf16* p, float v) { *p = (__bf16)v; }
-};
-template <> struct Elem<_Float16> {
-  static __device__ __forceinline__ float ld(const _Float16* p) { return (float)*p; }
-  static __device__ __forceinline__ void st(_Float16* p, float v) { *p = (_Float16)v; }
-};
-
-struct RnArgs {
-  // activations, element (b, c, p) at ptr + b * bs + c * cs + p * ps
-  const void *x, *f, *dy, *dn, *y_in;
-  void *y, *n, *dx, *df;
-  long x_bs, f_bs, dy_bs, dn_bs, yi_bs, y_bs, n_bs, dx_bs, df_bs;
-  long cs, ps;
-  const float *post_w, *post_b, *gate, *scale, *pre_w, *pre_b;
-  const float* stats_in;   // [4][B][P]
-  float* stats;            // [4][B][P] or null
-  float* rowsum;           // backward: [2][B][P], the two row means of the pre norm's gradient
-  float* part;             // backward: [5][workers][C] partial parameter gradients
-  float* part_gate;        // backward, gate kind 2 and S > 1: [B][S][C]
-  float* dgate;            // backward, gate kind 2 and S == 1: written directly
-  int post, pre, gate_kind, accumulate;
-  float eps;
-  int B, C, P;
-  int S, ipw;              // workers per image (ipw == 1), or images per worker (S == 1)
-};
-enum { Q_POST_W = 0, Q_POST_B = 1, Q_GATE = 2, Q_PRE_W = 3, Q_PRE_B = 4, Q_N = 5 };
-
-// ---- any number of channels -------------------------------------------------------------------------------------------
-// One workgroup per token (tokens layout, 256 threads along the channels) or per 64 pixels (planar, four waves along
-// the channels); nothing is kept between the passes over the channels, each reads its operands again.
-template <bool TOK>
-struct Sweep {
-  float* red;
-  // sum over the threads that share a token
-  __device__ __forceinline__ float sum(float v) const {
-    const int tid = threadIdx.x;
-    __syncthreads();
-    if (TOK) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-      if ((tid & 63) == 0) red[tid >> 6] = v;
-      __syncthreads();
-      return (red[0] + red[1]) + (red[2] + red[3]);
-    }
-    red[tid] = v;
-    __syncthreads();
-    const int l = tid & 63;
-    return (red[l] + red[64 + l]) + (red[128 + l] + red[192 + l]);
-  }
-};
-
-template <typename T, bool TOK>
-__global__ __launch_bounds__(256) void rn_fwd_sweep(const RnArgs a) {
-  __shared__ float red[256];
-  const Sweep<TOK> sw{red};
-  const int tid = threadIdx.x;
-  const long tiles = TOK ? a.P : (a.P + 63) / 64;
-  const int c0 = TOK ? tid : tid >> 6, dc = TOK ? 256 : 4;
-  const float inv = 1.0f / (float)a.C;
-  for (long t = blockIdx.x; t < tiles * a.B; t += gridDim.x) {
-    const long b = t / tiles, pt = t % tiles;
-    const long p = TOK ? pt : pt * 64 + (tid & 63);
-    const bool on = p < a.P;
-    const long o = (on ? p : 0) * a.ps;
-    const T* x = static_cast<const T*>(a.x) + b * a.x_bs + o;
-    const T* f = static_cast<const T*>(a.f) + b * a.f_bs + o;
-    T* y = static_cast<T*>(a.y) + b * a.y_bs + o;
-    T* n = static_cast<T*>(a.n) + (a.pre ? b * a.n_bs + o : 0);
-    const float s = a.scale ? a.scale[b] : 1.0f;
-    const float* gate = a.gate_kind == 2 ? a.gate + b * a.C : a.gate;
-    float mu0 = 0.f, rs0 = 0.f, mu1 = 0.f, rs1 = 0.f;
-    if (a.post) {
-      float q = 0.f;
-      if (a.post != 3) {
-        for (int c = c0; c < a.C; c += dc) q += Elem<T>::ld(f + c * a.cs);
-        mu0 = sw.sum(q) * inv;
-      }
-      q = 0.f;
-      for (int c = c0; c < a.C; c += dc) {
-        const float d = Elem<T>::ld(f + c * a.cs) - mu0;
-        q = fmaf(d, d, q);
-      }
-      rs0 = 1.0f / sqrtf(sw.sum(q) * inv + a.eps);
-    }
-    auto join = [&](int c) {
-      float u = Elem<T>::ld(f + c * a.cs);
-      if (a.post) {
-        u = (a.post == 1 ? u - mu0 : u) * rs0 * a.post_w[c];
-        if (a.post == 1 && a.post_b) u += a.post_b[c];
-      }
-      return fmaf(a.gate_kind ? s * gate[c] : s, u, Elem<T>::ld(x + c * a.cs));
-    };
-    if (a.pre) {
-      float q = 0.f;
-      if (a.pre != 3) {
-        for (int c = c0; c < a.C; c += dc) q += join(c);
-        mu1 = sw.sum(q) * inv;
-      }
-      q = 0.f;
-      for (int c = c0; c < a.C; c += dc) {
-        const float d = join(c) - mu1;
-        q = fmaf(d, d, q);
-      }
-      rs1 = 1.0f / sqrtf(sw.sum(q) * inv + a.eps);
-    }
-    if (on) {
-      for (int c = c0; c < a.C; c += dc) {      // y may be x and n may be f: a thread reads both before it writes
-        const float v = join(c);
-        Elem<T>::st(y + c * a.cs, v);
-        if (a.pre) {
-          float r = (a.pre == 1 ? v - mu1 : v) * rs1 * a.pre_w[c];
-          if (a.pre == 1 && a.pre_b) r += a.pre_b[c];
-          Elem<T>::st(n + c * a.cs, r);
-        }
-      }
-      if (a.stats && c0 == 0) {
-        const long bp = (long)a.B * a.P, at = b * a.P + p;
-        a.stats[at] = mu0;
-        a.stats[bp + at] = rs0;
-        a.stats[2 * bp + at] = mu1;
-        a.stats[3 * bp + at] = rs1;
-      }
-    }
-  }
-}
-
-// What the backward's element formulas need of one token.
-struct RowBwd {
-  float mu0, rs0, mu1, rs1, m1, m2, s;
-};
-
-// dyt of one element: dy + rs (g - [kind 1] mean g - c mean(g vh))
-__device__ __forceinline__ float rn_dyt(const RnArgs& a, const RowBwd& r, float dy, float dn, float y, float w) {
-  if (!a.pre) return dy;
-  return dy + r.rs1 * (dn * w - r.m1 - (y - r.mu1) * r.rs1 * r.m2);
-}
-
-template <typename T, bool TOK>
-__global__ __launch_bounds__(256) void rn_bwd_sweep(const RnArgs a) {
-  __shared__ float red[256];
-  const Sweep<TOK> sw{red};
-  const int tid = threadIdx.x;
-  const long tiles = TOK ? a.P : (a.P + 63) / 64;
-  const int c0 = TOK ? tid : tid >> 6, dc = TOK ? 256 : 4;
-  const float inv = 1.0f / (float)a.C;
-  const long bp = (long)a.B * a.P;
-  for (long t = blockIdx.x; t < tiles * a.B; t += gridDim.x) {
-    const long b = t / tiles, pt = t % tiles;
-    const long p = TOK ? pt : pt * 64 + (tid & 63);
-    const bool on = p < a.P;
-    const long o = (on ? p : 0) * a.ps, at = b * a.P + (on ? p : 0);
-    const T* dy = a.dy ? static_cast<const T*>(a.dy) + b * a.dy_bs + o : nullptr;
-    const T* dn = a.pre ? static_cast<const T*>(a.dn) + b * a.dn_bs + o : nullptr;
-    const T* y = a.pre ? static_cast<const T*>(a.y_in) + b * a.yi_bs + o : nullptr;
-    const T* f = a.post ? static_cast<const T*>(a.f) + b * a.f_bs + o : nullptr;
-    T* dx = static_cast<T*>(a.dx) + b * a.dx_bs + o;
-    T* df = static_cast<T*>(a.df) + b * a.df_bs + o;
-    const float* gate = a.gate_kind == 2 ? a.gate + b * a.C : a.gate;
-    RowBwd r{};
-    r.s = a.scale ? a.scale[b] : 1.0f;
-    if (a.post) {
-      r.mu0 = a.stats_in[at];
-      r.rs0 = a.stats_in[bp + at];
-    }
-    if (a.pre) {
-      r.mu1 = a.stats_in[2 * bp + at];
-      r.rs1 = a.stats_in[3 * bp + at];
-      const float m = a.pre == 1 ? r.mu1 : 0.f;
-      float s1 = 0.f, s2 = 0.f;
-      for (int c = c0; c < a.C; c += dc) {
-        const float g = Elem<T>::ld(dn + c * a.cs) * a.pre_w[c];
-        s1 += g;
-        s2 = fmaf(g, (Elem<T>::ld(y + c * a.cs) - m) * r.rs1, s2);
-      }
-      r.m1 = a.pre == 1 ? sw.sum(s1) * inv : 0.f;
-      r.m2 = sw.sum(s2) * inv;
-      if (on && c0 == 0) {
-        a.rowsum[at] = r.m1;
-        a.rowsum[bp + at] = r.m2;
-      }
-    }
-    auto dyt = [&](int c) {
-      return rn_dyt(a, r, dy ? Elem<T>::ld(dy + c * a.cs) : 0.f, a.pre ? Elem<T>::ld(dn + c * a.cs) : 0.f,
-                    a.pre ? Elem<T>::ld(y + c * a.cs) : 0.f, a.pre ? a.pre_w[c] : 0.f);
-    };
-    float t1 = 0.f, t2 = 0.f;
-    if (a.post) {
-      const float m = a.post == 1 ? r.mu0 : 0.f;
-      for (int c = c0; c < a.C; c += dc) {
-        const float g = dyt(c) * (a.gate_kind ? r.s * gate[c] : r.s) * a.post_w[c];
-        t1 += g;
-        t2 = fmaf(g, (Elem<T>::ld(f + c * a.cs) - m) * r.rs0, t2);
-      }
-      t1 = a.post == 1 ? sw.sum(t1) * inv : 0.f;
-      t2 = sw.sum(t2) * inv;
-    }
-    if (on)
-      for (int c = c0; c < a.C; c += dc) {
-        const float d = dyt(c);
-        float du = d * (a.gate_kind ? r.s * gate[c] : r.s);
-        if (a.post) du = r.rs0 * (du * a.post_w[c] - t1 - (Elem<T>::ld(f + c * a.cs) - r.mu0) * r.rs0 * t2);
-        Elem<T>::st(dx + c * a.cs, d);
-        Elem<T>::st(df + c * a.cs, du);
-      }
-  }
-}
-
-// The parameter gradients of the sweep form: one pass more over the operands, a workgroup per 64 channels and worker
-// (tokens: lanes along the channels, waves along the rows; planar: a wave per channel, lanes along the pixels).
-template <typename T, bool TOK>
-__global__ __launch_bounds__(256) void rn_bwd_params_sweep(const RnArgs a) {
-  __shared__ float red[Q_N][256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int worker = blockIdx.y;
-  const int b0 = a.S > 1 ? worker / a.S : worker * a.ipw, b1 = min(a.B, a.S > 1 ? b0 + 1 : b0 + a.ipw);
-  const int slab = a.S > 1 ? worker % a.S : 0;
-  const int per = (a.P + a.S - 1) / a.S, p0 = min(a.P, slab * per), p1 = min(a.P, p0 + per);
-  const long bp = (long)a.B * a.P;
-  const int c = blockIdx.x * (TOK ? 64 : 4) + (TOK ? lane : wave);
-  const bool on = c < a.C;
-  const int cc = on ? c : 0;
-  float acc[Q_N] = {0.f, 0.f, 0.f, 0.f, 0.f};
-  // per-channel sums across the threads that share the channel
-  auto total = [&](float v, float* buf) {
-    if (!TOK) {
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-      return v;
-    }
-    __syncthreads();
-    buf[tid] = v;
-    __syncthreads();
-    return (buf[lane] + buf[64 + lane]) + (buf[128 + lane] + buf[192 + lane]);
-  };
-  const bool writer = on && (TOK ? wave == 0 : lane == 0);
-  for (int b = b0; b < b1; ++b) {
-    const float s = a.scale ? a.scale[b] : 1.0f;
-    const float gt = a.gate_kind == 2 ? a.gate[(long)b * a.C + cc] : a.gate_kind ? a.gate[cc] : 1.0f;
-    const float w1 = a.pre ? a.pre_w[cc] : 0.f, w0 = a.post ? a.post_w[cc] : 1.f;
-    const float b0v = a.post == 1 && a.post_b ? a.post_b[cc] : 0.f;
-    float gacc = 0.f;
-    for (int p = p0 + (TOK ? wave : lane); p < p1; p += TOK ? 4 : 64) {
-      const long o = p * a.ps + cc * a.cs, at = (long)b * a.P + p;
-      RowBwd r{};
-      float dnv = 0.f, yv = 0.f;
-      if (a.pre) {
-        r.mu1 = a.stats_in[2 * bp + at];
-        r.rs1 = a.stats_in[3 * bp + at];
-        r.m1 = a.rowsum[at];
-        r.m2 = a.rowsum[bp + at];
-        dnv = Elem<T>::ld(static_cast<const T*>(a.dn) + b * a.dn_bs + o);
-        yv = Elem<T>::ld(static_cast<const T*>(a.y_in) + b * a.yi_bs + o);
-        acc[Q_PRE_W] = fmaf(dnv, (a.pre == 1 ? yv - r.mu1 : yv) * r.rs1, acc[Q_PRE_W]);
-        acc[Q_PRE_B] += dnv;
-      }
-      if (!a.post && !a.gate_kind) continue;
-      const float d = rn_dyt(a, r, a.dy ? Elem<T>::ld(static_cast<const T*>(a.dy) + b * a.dy_bs + o) : 0.f, dnv, yv, w1) * s;
-      float u = Elem<T>::ld(static_cast<const T*>(a.f) + b * a.f_bs + o);
-      if (a.post) {
-        u = (a.post == 1 ? u - a.stats_in[at] : u) * a.stats_in[bp + at];
-        acc[Q_POST_W] = fmaf(d * gt, u, acc[Q_POST_W]);
-        acc[Q_POST_B] += d * gt;
-        u = fmaf(u, w0, b0v);
-      }
-      gacc = fmaf(d, u, gacc);
-    }
-    if (a.gate_kind == 2) {
-      const float g = total(gacc, red[Q_GATE]);
-      if (writer) {
-        if (a.S > 1) a.part_gate[((long)b * a.S + slab) * a.C + c] = g;
-        else if (a.dgate) a.dgate[(long)b * a.C + c] = a.accumulate ? a.dgate[(long)b * a.C + c] + g : g;
-      }
-    } else {
-      acc[Q_GATE] += gacc;
-    }
-  }
-  const long workers = gridDim.y;
-#pragma unroll
-  for (int q = 0; q < Q_N; ++q) {
-    const float v = total(acc[q], red[q]);
-    if (writer) a.part[((long)q * workers + worker) * a.C + c] = v;
-  }
-}
-
-// out[g][c] (+)= sum over rows r of part[g][r][c], rows in order per thread, then the row lanes in order, in 64 bits.
-// blockIdx.y: quantity; a null out skips it.
-struct ReduceArgs {
-  const float* part[Q_N];
-  float* out[Q_N];
-  long rows, C;
-  int accumulate;
-};
-__global__ __launch_bounds__(1024) void rn_reduce(const ReduceArgs a) {
-  __shared__ double red[32][33];
-  const float* part = a.part[blockIdx.y] + (long)blockIdx.z * a.rows * a.C;
-  float* out = a.out[blockIdx.y] + (long)blockIdx.z * a.C;
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  const long c = (long)blockIdx.x * 32 + cl;
-  double t = 0.0;
-  if (c < a.C)
-    for (long r = rl; r < a.rows; r += 32) t += (double)part[r * a.C + c];
-  red[rl][cl] = t;
-  __syncthreads();
-  if (rl == 0 && c < a.C) {
-    double v = 0.0;
-#pragma unroll
-    for (int r = 0; r < 32; ++r) v += red[r][cl];
-    out[c] = a.accumulate ? (float)((double)out[c] + v) : (float)v;
-  }
-}
 
 // ---- host -------------------------------------------------------------------------------------------------------------
 template <typename F>
@@ -408,48 +90,141 @@ void set_layout(RnArgs& a, int layout) {
   a.ps = layout == JIRF_LAYOUT_TOKENS ? a.C : 1;
 }
 
-#define RN_DISPATCH(dtype, tok, KERNEL, grid, block, s, args)                                                  \
-  do {                                                                                                         \
-    if (dtype == JIRF_F32) {                                                                                   \
-      if (tok) hipLaunchKernelGGL((KERNEL<float, true>), grid, block, 0, s, args);                             \
-      else hipLaunchKernelGGL((KERNEL<float, false>), grid, block, 0, s, args);                                \
-    } else if (dtype == JIRF_BF16) {                                                                           \
-      if (tok) hipLaunchKernelGGL((KERNEL<__bf16, true>), grid, block, 0, s, args);                            \
-      else hipLaunchKernelGGL((KERNEL<__bf16, false>), grid, block, 0, s, args);                               \
-    } else {                                                                                                   \
-      if (tok) hipLaunchKernelGGL((KERNEL<_Float16, true>), grid, block, 0, s, args);                          \
-      else hipLaunchKernelGGL((KERNEL<_Float16, false>), grid, block, 0, s, args);                             \
-    }                                                                                                          \
+#define RN_TYPE(dtype, CALL)                          \
+  do {                                                \
+    if (dtype == JIRF_F32) CALL<float> RN_ARGS;       \
+    else if (dtype == JIRF_BF16) CALL<__bf16> RN_ARGS; \
+    else CALL<_Float16> RN_ARGS;                      \
   } while (0)
 
-unsigned sweep_grid(bool tok, int B, int P) {
-  const long tiles = (tok ? (long)P : ((long)P + 63) / 64) * B;
-  return (unsigned)std::min<long>(tiles, 1 << 16);
-}
-
-// Workers of the parameter gradients: at least 64 pixels each, about 256 of them.
-void bwd_workers(RnArgs& a) {
-  const int want = 256;
-  if (a.B >= want) {
-    a.S = 1;
-    a.ipw = (a.B + want - 1) / want;
+// Which kernel serves (layout, type, B, C, P): the register form wherever a workgroup of 512 threads can hold a token (or a
+// few pixels) of all channels, the sweep form beyond.
+RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
+  RnForm f{};
+  f.tok = layout == JIRF_LAYOUT_TOKENS;
+  const int vec = f.tok ? (dtype == JIRF_F32 ? 4 : 8) : 4;
+  a.tiles = a.P;
+  a.S = a.ipw = 1;
+  long per_block = 1;                  // workers of a workgroup
+  if (f.tok) {
+    // eight channels per thread; sixteen where eight would need more than 512 threads
+    const int threads8 = (a.C + 7) / 8;
+    f.nv = 8 / vec;
+    if (threads8 <= 64) {
+      f.lanes = threads8 <= 8 ? 8 : threads8 <= 16 ? 16 : threads8 <= 32 ? 32 : 64;
+      f.threads = 256;
+      per_block = f.threads / f.lanes;
+    } else if (threads8 <= 512) {
+      f.threads = (threads8 + 63) / 64 * 64;
+    } else if (a.C <= 8192) {
+      f.nv *= 2;
+      f.threads = ((a.C + 15) / 16 + 63) / 64 * 64;
+    } else {
+      f.lanes = -1;
+    }
   } else {
-    a.ipw = 1;
-    a.S = (int)std::max<long>(1, std::min<long>((a.P + 63) / 64, want / a.B));
+    // four channels of four pixels per thread: as many pixel lanes (of 32) as the channels leave room for in 256 threads,
+    // more threads only to keep eight lanes (a 128-byte line of fp32) or, past that, any
+    const int rows = (a.C + 3) / 4;
+    f.nv = 4;
+    f.lanes = 32;
+    while (f.lanes > 8 && f.lanes * rows > 256) f.lanes >>= 1;
+    while (f.lanes > 2 && f.lanes * rows > 512) f.lanes >>= 1;
+    // no wider than the plane, and narrower while the tiles leave CUs idle
+    while (f.lanes > 4 && (f.lanes * 2 >= a.P || ((long)a.P + f.lanes * 4 - 1) / (f.lanes * 4) * a.B < 256)) f.lanes >>= 1;
+    f.threads = std::max(64, (f.lanes * rows + 63) / 64 * 64);
+    if (f.threads > 512) f.lanes = -1;
+    else a.tiles = (int)(((long)a.P + f.lanes * 4 - 1) / (f.lanes * 4));
   }
+  // Workers: enough workgroups to fill the chip several times over (forward), or about twice (backward: each leaves a row
+  // of partial sums per parameter).
+  if (f.lanes < 0) a.tiles = (int)(((long)a.P + 63) / 64);
+  const long want = (f.lanes < 0 ? 256 : backward ? 512 : 2048) * per_block;
+  if (a.B >= want) {
+    a.ipw = (int)((a.B + want - 1) / want);
+    a.per = a.tiles;
+  } else {
+    const long S = std::max<long>(1, std::min<long>(a.tiles, want / a.B));
+    a.per = (int)((a.tiles + S - 1) / S);
+    a.S = (int)((a.tiles + a.per - 1) / a.per);
+  }
+  const long workers = a.S > 1 ? (long)a.B * a.S : ((long)a.B + a.ipw - 1) / a.ipw;
+  f.blocks = (unsigned)((workers + per_block - 1) / per_block);
+  a.part_rows = f.blocks;
+  return f;
 }
-long n_workers(const RnArgs& a) { return a.S > 1 ? (long)a.B * a.S : ((long)a.B + a.ipw - 1) / a.ipw; }
 
 struct BwdWork {
   long rowsum, part, part_gate, total;   // floats
 };
-BwdWork bwd_work(const RnArgs& a) {
+BwdWork bwd_work(const RnArgs& a, const RnForm& f) {
   BwdWork w{};
-  w.rowsum = a.pre ? 2l * a.B * a.P : 0;
-  w.part = (long)Q_N * n_workers(a) * a.C;
+  w.rowsum = f.lanes < 0 && a.pre ? 2l * a.B * a.P : 0;
+  w.part = (long)RN_Q_N * a.part_rows * a.C;
   w.part_gate = a.gate_kind == 2 && a.S > 1 ? (long)a.B * a.S * a.C : 0;
   w.total = w.rowsum + w.part + w.part_gate;
   return w;
+}
+
+// Adds the partial sums up, rows in order per thread and the 32 row lanes in order, in 64 bits.  blockIdx.y 0: the branch (G1,
+// G0 -> dpost_w, dpost_b, dgate), 1: the norm before the next block.
+struct ReduceArgs {
+  const float* part;
+  long rows, C;
+  float *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
+  const float *gate, *post_w, *post_b;   // gate: null with a gate per image (its factors are in the sums already)
+  int has_post, accumulate;
+};
+__device__ __forceinline__ double reduce_column(const float* part, long rows, long C, long c, double (*red)[33]) {
+  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+  double t = 0.0;
+  if (c < C)
+    for (long r = rl; r < rows; r += 32) t += (double)part[r * C + c];
+  __syncthreads();
+  red[rl][cl] = t;
+  __syncthreads();
+  double v = 0.0;
+  if (rl == 0)
+#pragma unroll
+    for (int r = 0; r < 32; ++r) v += red[r][cl];
+  return v;
+}
+__device__ __forceinline__ void reduce_out(float* out, long c, double v, int accumulate) {
+  if (out) out[c] = accumulate ? (float)((double)out[c] + v) : (float)v;
+}
+__global__ __launch_bounds__(1024) void rn_reduce(const ReduceArgs a) {
+  __shared__ double red[32][33];
+  const long c = (long)blockIdx.x * 32 + (threadIdx.x & 31);
+  const bool writer = threadIdx.x < 32 && c < a.C;
+  const long plane = a.rows * a.C;
+  if (blockIdx.y == 0) {
+    if (!a.dpost_w && !a.dpost_b && !a.dgate) return;
+    const double g1 = reduce_column(a.part + RN_Q_G1 * plane, a.rows, a.C, c, red);
+    const bool g0_used = a.dpost_b || (a.dgate && a.post_b);
+    const double g0 = g0_used ? reduce_column(a.part + RN_Q_G0 * plane, a.rows, a.C, c, red) : 0.0;
+    if (!writer) return;
+    const double g = a.gate ? (double)a.gate[c] : 1.0;
+    reduce_out(a.dpost_w, c, g * g1, a.accumulate);
+    reduce_out(a.dpost_b, c, g * g0, a.accumulate);
+    reduce_out(a.dgate, c, a.has_post ? a.post_w[c] * g1 + (a.post_b ? a.post_b[c] * g0 : 0.0) : g1, a.accumulate);
+  } else {
+    if (a.dpre_w) {
+      const double v = reduce_column(a.part + RN_Q_PRE_W * plane, a.rows, a.C, c, red);
+      if (writer) reduce_out(a.dpre_w, c, v, a.accumulate);
+    }
+    if (a.dpre_b) {
+      const double v = reduce_column(a.part + RN_Q_PRE_B * plane, a.rows, a.C, c, red);
+      if (writer) reduce_out(a.dpre_b, c, v, a.accumulate);
+    }
+  }
+}
+// dgate [B][C] from the [B][S][C] sums of a gate per image
+__global__ __launch_bounds__(1024) void rn_reduce_gate(const float* __restrict__ part, long S, long C, float* __restrict__ dgate,
+                                                       int accumulate) {
+  __shared__ double red[32][33];
+  const long c = (long)blockIdx.x * 32 + (threadIdx.x & 31);
+  const double v = reduce_column(part + (long)blockIdx.y * S * C, S, C, c, red);
+  if (threadIdx.x < 32 && c < C) reduce_out(dgate + (long)blockIdx.y * C, c, v, accumulate);
 }
 
 }  // namespace
@@ -484,10 +259,12 @@ int jirf_train_residual_norm(const void* x, long x_bs, const void* f, long f_bs,
     a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.pre_b = pre_b; a.gate = gate; a.scale = scale;
     a.eps = eps; a.stats = stats; a.B = B; a.C = C; a.P = P;
     set_layout(a, layout);
-    const bool tok = layout == JIRF_LAYOUT_TOKENS;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Scope sc("train_residual_norm", 10.0 * B * C * (double)P, (dtype == JIRF_F32 ? 4.0 : 2.0) * B * C * (double)P * (pre_kind ? 4 : 3), s);
-    RN_DISPATCH(dtype, tok, rn_fwd_sweep, dim3(sweep_grid(tok, B, P)), dim3(256), s, a);
+    const RnForm f_ = choose_form(a, dtype, layout, false);
+#define RN_ARGS (a, f_, s)
+    RN_TYPE(dtype, rn_launch_fwd);
+#undef RN_ARGS
     JIRF_HIP_CHECK(hipGetLastError());
     return JIRF_OK;
   });
@@ -499,8 +276,8 @@ long jirf_train_residual_norm_bwd_work_floats(int dtype, int layout, int post_ki
     return -1;
   RnArgs a{};
   a.post = post_kind; a.pre = pre_kind; a.gate_kind = gate_kind; a.B = B; a.C = C; a.P = P;
-  bwd_workers(a);
-  return bwd_work(a).total;
+  const RnForm form = choose_form(a, dtype, layout, true);
+  return bwd_work(a, form).total;
 }
 
 int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, long dn_bs, const void* y, long y_bs, const void* f,
@@ -540,37 +317,30 @@ int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, lon
     a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.gate = gate; a.scale = scale;
     a.stats_in = stats; a.accumulate = accumulate; a.B = B; a.C = C; a.P = P;
     set_layout(a, layout);
-    bwd_workers(a);
-    const BwdWork wk = bwd_work(a);
-    a.rowsum = work;
-    a.part = work + wk.rowsum;
-    a.part_gate = a.part + wk.part;
-    a.dgate = dgate;
-    const bool tok = layout == JIRF_LAYOUT_TOKENS;
+    const RnForm form = choose_form(a, dtype, layout, true);
+    const BwdWork wk = bwd_work(a, form);
+    const bool branch = post_kind || gate_kind;
+    const bool params = dpost_w || dpost_b || dgate || dpre_w || dpre_b;
+    if (work) {
+      a.rowsum = work;
+      a.part = params ? work + wk.rowsum : nullptr;
+      a.part_gate = dgate ? work + wk.rowsum + wk.part : nullptr;
+    }
+    a.dgate = gate_kind == 2 ? dgate : nullptr;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int reads = 1 + (pre_kind ? 2 : 0) + (post_kind || gate_kind ? 1 : 0);
+    const int reads = 1 + (pre_kind ? 2 : 0) + (branch ? 1 : 0);
+    const int mode = !branch ? RN_BWD_STREAM : gate_kind == 2 ? RN_BWD_IMAGE_GATE : RN_BWD_BRANCH;
     Scope sc("train_residual_norm_bwd", 25.0 * B * C * (double)P, (dtype == JIRF_F32 ? 4.0 : 2.0) * B * C * (double)P * (reads + 2), s);
-    RN_DISPATCH(dtype, tok, rn_bwd_sweep, dim3(sweep_grid(tok, B, P)), dim3(256), s, a);
-    if (dpost_w || dpost_b || dgate || dpre_w || dpre_b) {
-      const long workers = n_workers(a);
-      RN_DISPATCH(dtype, tok, rn_bwd_params_sweep, dim3((unsigned)((C + (tok ? 63 : 3)) / (tok ? 64 : 4)), (unsigned)workers), dim3(256), s, a);
-      ReduceArgs r{};
-      float* outs[Q_N] = {dpost_w, dpost_b, gate_kind == 1 ? dgate : nullptr, dpre_w, dpre_b};
-      int nq = 0;
-      for (int q = 0; q < Q_N; ++q)
-        if (outs[q]) {
-          r.part[nq] = a.part + (long)q * workers * C;
-          r.out[nq++] = outs[q];
-        }
-      r.rows = workers; r.C = C; r.accumulate = accumulate;
-      if (nq) hipLaunchKernelGGL(rn_reduce, dim3((unsigned)((C + 31) / 32), nq, 1), dim3(1024), 0, s, r);
-      if (gate_kind == 2 && dgate && a.S > 1) {
-        ReduceArgs g{};
-        g.part[0] = a.part_gate;
-        g.out[0] = dgate;
-        g.rows = a.S; g.C = C; g.accumulate = accumulate;
-        hipLaunchKernelGGL(rn_reduce, dim3((unsigned)((C + 31) / 32), 1, (unsigned)B), dim3(1024), 0, s, g);
-      }
+#define RN_ARGS (a, form, mode, params, s)
+    RN_TYPE(dtype, rn_launch_bwd);
+#undef RN_ARGS
+    if (params) {
+      const ReduceArgs r{a.part, a.part_rows, C, dpost_w, dpost_b, gate_kind == 1 ? dgate : nullptr, dpre_w, dpre_b,
+                         gate_kind == 1 ? gate : nullptr, post_w, post_kind == 1 ? post_b : nullptr, post_kind, accumulate};
+      hipLaunchKernelGGL(rn_reduce, dim3((unsigned)((C + 31) / 32), 2), dim3(1024), 0, s, r);
+      if (gate_kind == 2 && dgate && a.S > 1)
+        hipLaunchKernelGGL(rn_reduce_gate, dim3((unsigned)((C + 31) / 32), (unsigned)B), dim3(1024), 0, s, a.part_gate, (long)a.S,
+                           (long)C, dgate, accumulate);
     }
     JIRF_HIP_CHECK(hipGetLastError());
     return JIRF_OK;
