@@ -20,6 +20,7 @@ struct RnArgs {
   float* part_gate;        // backward, gate kind 2 and S > 1: [B][S][C]
   float* dgate;            // backward, gate kind 2 and S == 1: written directly
   long part_rows;
+  int wanted;              // bit q: the sums RN_Q_* q are needed
   int post, pre, gate_kind, accumulate;
   float eps;
   int B, C, P;
@@ -63,36 +64,30 @@ template <> struct Elem<_Float16> {
   static __device__ __forceinline__ void st(_Float16* p, float v) { *p = (_Float16)v; }
 };
 
-// VEC consecutive elements as loaded, read and written at the alignment of one element (rows of odd length, channel slices:
-// the memory instructions take any 2- or 4-byte address).
+// VEC consecutive elements, read and written at the alignment of one element (rows of odd length, channel slices: the
+// memory instructions take any 2- or 4-byte address), `off` bytes into an image.
 template <typename T, int VEC> struct Pack {
   typedef T V __attribute__((ext_vector_type(VEC)));
   typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   V v;
-  // n < VEC: only the first n exist
-  __device__ __forceinline__ void load(const T* p, int n) {
-    if (n >= VEC) {
-      v = *reinterpret_cast<const VU*>(p);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = i < n ? p[i] : (T)0.f;
-    }
-  }
+  __device__ __forceinline__ void load(const char* image, unsigned off) { v = *reinterpret_cast<const VU*>(image + off); }
   __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
 };
+// the last `own` of VEC values
 template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(T* p, int n, const float* f) {
+__device__ __forceinline__ void store_vec(char* image, unsigned off, int own, const float* f) {
   typedef T V __attribute__((ext_vector_type(VEC)));
   typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   V v;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) v[i] = (T)f[i];
-  if (n >= VEC) {
+  T* p = reinterpret_cast<T*>(image + off);
+  if (own == VEC) {
     *reinterpret_cast<VU*>(p) = v;
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
-      if (i < n) p[i] = v[i];
+      if (i >= VEC - own) p[i] = v[i];
   }
 }
 
@@ -104,6 +99,10 @@ constexpr int RN_LANE_T = 256;    // threads of a workgroup whose waves hold sev
 // read once.  tokens: a tile is one token, a vector VEC consecutive channels, and the token's threads are L lanes of a
 // wave (a worker per lane group) or the workgroup (L == 0).  planar: a tile is L * VEC pixels of all channels, a vector VEC
 // consecutive pixels of one channel; L lanes run along the pixels, the other threads along the channels.
+// A vector that would reach past the channels (the pixels) is moved back to end at the last one, so every load is whole and
+// none branches; the elements it then shares with its neighbour belong to the neighbour: they are left out of sums and
+// stores.  A thread without a channel repeats the last one and owns nothing.  Needs C >= VEC (tokens) or P >= VEC (planar),
+// and less than 2^32 bytes in an image.
 template <typename T, bool TOK, int L, int NV, int VEC>
 struct Tile {
   static constexpr int NS = TOK ? 1 : VEC;       // statistics per thread: its token's, or one per pixel of its vector
@@ -113,8 +112,8 @@ struct Tile {
   float* red;                                    // LDS of two reductions
   int buf;
   int ch, nch, pl;                               // position among the token's threads, their number, pixel lane
-  int cnt[NV];                                   // tokens: channels of each vector that exist; planar: 0 or VEC
-  long off[NV];                                  // offset of each vector's first element from the tile's first
+  int own[NV];                                   // tokens: elements of each vector that are its own; planar: 1 or 0
+  unsigned off[NV];                              // bytes from the token's first channel / from the image's first pixel 0
 
   static constexpr int RED = TOK ? (L ? 1 : 2 * 8 * 2) : 2 * 8 * L * 2 * VEC;
 
@@ -131,48 +130,62 @@ struct Tile {
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = channel(j);
       if (TOK) {
-        cnt[j] = max(0, min(VEC, a.C - c));
-        off[j] = c;
+        const int c = (j * nch + ch) * VEC;
+        own[j] = max(0, min(VEC, a.C - c));
+        off[j] = (unsigned)channel(j) * sizeof(T);
       } else {
-        cnt[j] = c < a.C ? VEC : 0;
-        off[j] = (long)c * a.P + pl * VEC;
+        own[j] = j * nch + ch < a.C;
+        off[j] = (unsigned)channel(j) * (unsigned)a.P * (unsigned)sizeof(T);
       }
     }
   }
-  __device__ __forceinline__ int channel(int j) const { return TOK ? (j * nch + ch) * VEC : j * nch + ch; }
-  // elements of vector j inside tile t
-  __device__ __forceinline__ int count(int j, int t) const {
-    if (TOK) return cnt[j];
-    const long left = (long)a.P - ((long)t * L + pl) * VEC;
-    return cnt[j] ? (int)min(left, (long)VEC) : 0;
+  // first channel of vector j as loaded
+  __device__ __forceinline__ int channel(int j) const {
+    return TOK ? min((j * nch + ch) * VEC, a.C - VEC) : min(j * nch + ch, a.C - 1);
   }
-  __device__ __forceinline__ bool exists(int j, int v) const { return TOK ? v < cnt[j] : cnt[j] > 0; }
-  __device__ __forceinline__ long origin(int b, long bs, int t) const {
-    return b * bs + (TOK ? (long)t * a.C : (long)t * (L * VEC));
+  __device__ __forceinline__ bool exists(int j, int v) const { return TOK ? v >= VEC - own[j] : own[j] != 0; }
+  // whether an element of a tile with px own pixels is the thread's own
+  __device__ __forceinline__ bool mine(int j, int v, int px) const { return exists(j, v) && (TOK || v >= VEC - px); }
+  // first pixel of this lane's vector in tile t as loaded, and how many (the last ones) are its own
+  __device__ __forceinline__ int pixel(int t) const { return TOK ? t : (int)min(((long)t * L + pl) * VEC, (long)a.P - VEC); }
+  __device__ __forceinline__ int own_pixels(int t) const {
+    return TOK ? 1 : (int)max(0l, min((long)VEC, (long)a.P - ((long)t * L + pl) * VEC));
   }
-  __device__ __forceinline__ void load(const T* base, int t, Vec (&r)[NV]) const {
+  __device__ __forceinline__ unsigned start(int t) const {
+    return (TOK ? (unsigned)t * (unsigned)a.C : (unsigned)pixel(t)) * (unsigned)sizeof(T);
+  }
+  static __device__ __forceinline__ const char* image(const void* p, long bs, int b) {
+    return reinterpret_cast<const char*>(static_cast<const T*>(p) + b * bs);
+  }
+  __device__ __forceinline__ void load(const char* img, unsigned st, Vec (&r)[NV]) const {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) r[j].load(img, st + off[j]);
+  }
+  __device__ __forceinline__ void store(void* p, long bs, int b, unsigned st, int px, const float (&f)[NV][VEC]) const {
+    char* img = const_cast<char*>(image(p, bs, b));
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int n = count(j, t);
-      if (n > 0) r[j].load(base + off[j], n);
-      else r[j].v = typename Vec::V(0);
+      const int n = TOK ? own[j] : own[j] ? px : 0;
+      if (n > 0) store_vec<T, VEC>(img, st + off[j], n, f[j]);
     }
   }
-  __device__ __forceinline__ void store(T* base, int t, const float (&f)[NV][VEC]) const {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int n = count(j, t);
-      if (n > 0) store_vec<T, VEC>(base + off[j], n, f[j]);
-    }
-  }
-  // a [C] array in the thread's channels; `none` where there is no channel or no array
+  // a [C] array in the thread's channels; `none` for a channel that is not its own, or without an array
   __device__ __forceinline__ void params(const float* p, float none, float (&r)[NV][NP]) const {
+    typedef float F __attribute__((ext_vector_type(NP), aligned(4)));
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
 #pragma unroll
-      for (int v = 0; v < NP; ++v) r[j][v] = p && exists(j, v) ? p[channel(j) + v] : none;
+      for (int v = 0; v < NP; ++v) r[j][v] = none;
+      if (!p) continue;
+      if constexpr (NP == 1) {
+        r[j][0] = own[j] ? p[channel(j)] : none;
+      } else {
+        const F q = *reinterpret_cast<const F*>(p + channel(j));
+#pragma unroll
+        for (int v = 0; v < NP; ++v) r[j][v] = exists(j, v) ? q[v] : none;
+      }
+    }
   }
   // Sums v[0..N) over the threads of the token.  Lanes first, then the waves in order through LDS; two buffers in turn, so
   // one barrier per reduction is enough.
@@ -214,7 +227,7 @@ struct Tile {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) mu[TOK ? 0 : i] += v[j][i];       // (absent elements are 0)
+        for (int i = 0; i < VEC; ++i) mu[TOK ? 0 : i] += exists(j, i) ? v[j][i] : 0.f;
       reduce<NS>(mu);
 #pragma unroll
       for (int s = 0; s < NS; ++s) mu[s] *= inv;
@@ -267,13 +280,11 @@ __global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
   ti.range(ti.worker(), b0, b1, t0, t1, slab);
   if (b0 >= b1 || t0 >= t1) return;           // (uniform over the threads of a worker, and a worker's barriers are its own)
   float pw[NV][NP], pb[NV][NP], gw[NV][NP], gb[NV][NP];
+  Vec xn[NV], fn[NV];
+  ti.load(Ti::image(a.f, a.f_bs, b0), ti.start(t0), fn);
+  ti.load(Ti::image(a.x, a.x_bs, b0), ti.start(t0), xn);
   ti.params(a.pre ? a.pre_w : nullptr, 0.f, pw);
   ti.params(a.pre == 1 ? a.pre_b : nullptr, 0.f, pb);
-  const T* xp = static_cast<const T*>(a.x);
-  const T* fp = static_cast<const T*>(a.f);
-  Vec xn[NV], fn[NV];
-  ti.load(fp + ti.origin(b0, a.f_bs, t0), t0, fn);
-  ti.load(xp + ti.origin(b0, a.x_bs, t0), t0, xn);
   int gate_of = -1;
   for (int b = b0; b < b1; ++b) {
     if (gate_of < 0 || a.gate_kind == 2) {
@@ -302,9 +313,11 @@ __global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
       }
       const int bn = t + 1 < t1 ? b : b + 1, tn = t + 1 < t1 ? t + 1 : t0;
       if (bn < b1) {
-        ti.load(fp + ti.origin(bn, a.f_bs, tn), tn, fn);
-        ti.load(xp + ti.origin(bn, a.x_bs, tn), tn, xn);
+        ti.load(Ti::image(a.f, a.f_bs, bn), ti.start(tn), fn);
+        ti.load(Ti::image(a.x, a.x_bs, bn), ti.start(tn), xn);
       }
+      const unsigned st = ti.start(t);
+      const int px = ti.own_pixels(t);
       float v[NV][VEC], mu0[NS], rs0[NS], mu1[NS], rs1[NS];
 #pragma unroll
       for (int i = 0; i < NS; ++i) mu0[i] = rs0[i] = mu1[i] = rs1[i] = 0.f;
@@ -323,8 +336,8 @@ __global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
       for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-          v[j][i] = ti.exists(j, i) ? fmaf(s, fmaf(v[j][i], gw[j][TOK ? i : 0], gb[j][TOK ? i : 0]), xv[j].at(i)) : 0.f;
-      ti.store(static_cast<T*>(a.y) + ti.origin(b, a.y_bs, t), t, v);
+          v[j][i] = fmaf(s, fmaf(v[j][i], gw[j][TOK ? i : 0], gb[j][TOK ? i : 0]), xv[j].at(i));
+      ti.store(a.y, a.y_bs, b, st, px, v);
       if (a.pre) {
         ti.statistics(v, a.pre, mu1, rs1);
 #pragma unroll
@@ -332,19 +345,18 @@ __global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
             v[j][i] = fmaf((a.pre == 1 ? v[j][i] - mu1[TOK ? 0 : i] : v[j][i]) * rs1[TOK ? 0 : i], pw[j][TOK ? i : 0], pb[j][TOK ? i : 0]);
-        ti.store(static_cast<T*>(a.n) + ti.origin(b, a.n_bs, t), t, v);
+        ti.store(a.n, a.n_bs, b, st, px, v);
       }
       if (a.stats && ti.ch == 0) {
         const long bp = (long)a.B * a.P;
-        const long p0 = TOK ? t : ((long)t * L + ti.pl) * VEC;
-        float* st = a.stats + (long)b * a.P + p0;
+        float* sp = a.stats + (long)b * a.P + ti.pixel(t);
 #pragma unroll
         for (int i = 0; i < NS; ++i)
-          if (p0 + i < a.P) {
-            st[i] = mu0[i];
-            st[bp + i] = rs0[i];
-            st[2 * bp + i] = mu1[i];
-            st[3 * bp + i] = rs1[i];
+          if (i >= NS - px) {
+            sp[i] = mu0[i];
+            sp[bp + i] = rs0[i];
+            sp[2 * bp + i] = mu1[i];
+            sp[3 * bp + i] = rs1[i];
           }
       }
     }
@@ -360,6 +372,8 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
   constexpr int NS = Ti::NS, NP = Ti::NP;
   constexpr bool BR = MODE != RN_BWD_STREAM, IG = MODE == RN_BWD_IMAGE_GATE;
   constexpr int EW = NV * NP;                                  // channels of a thread
+  // the next tile's operands are fetched ahead where the registers (256 per thread) have room for two tiles
+  constexpr bool PF = !(BR && NV * VEC == 16 && (sizeof(T) == 4 || IG));
   __shared__ float lds[Ti::RED];
   __shared__ float wsum[TOK && L ? RN_LANE_T / 64 * L * EW : 1];
   Ti ti(a, lds);
@@ -378,41 +392,64 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
 #pragma unroll
     for (int i = 0; i < NP; ++i) img[0][j][i] = img[1][j][i] = 0.f;
   float pw[NV][NP], gw[NV][NP];
-  ti.params(a.pre ? a.pre_w : nullptr, 0.f, pw);
-  const T* dyp = static_cast<const T*>(a.dy);
-  const T* dnp = static_cast<const T*>(a.dn);
-  const T* yp = static_cast<const T*>(a.y_in);
-  const T* fp = static_cast<const T*>(a.f);
   const float inv = 1.0f / (float)a.C;
   const long bp = (long)a.B * a.P;
+  // the operands of the next tile, and its statistics
   Vec dyn[NV], dnn[NV], yn[NV], fn[NV];
+  float sn[4][NS];
   auto fetch = [&](int b, int t) {
-    if (a.dy) ti.load(dyp + ti.origin(b, a.dy_bs, t), t, dyn);
+    const unsigned st = ti.start(t);
+    const float* sp = a.stats_in + (long)b * a.P + ti.pixel(t);
     if (a.pre) {
-      ti.load(dnp + ti.origin(b, a.dn_bs, t), t, dnn);
-      ti.load(yp + ti.origin(b, a.yi_bs, t), t, yn);
+      ti.load(Ti::image(a.dn, a.dn_bs, b), st, dnn);
+      ti.load(Ti::image(a.y_in, a.yi_bs, b), st, yn);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        sn[2][i] = sp[2 * bp + i];
+        sn[3][i] = sp[3 * bp + i];
+      }
     }
-    if (BR) ti.load(fp + ti.origin(b, a.f_bs, t), t, fn);
+    if (a.dy) ti.load(Ti::image(a.dy, a.dy_bs, b), st, dyn);
+    if (BR) {
+      ti.load(Ti::image(a.f, a.f_bs, b), st, fn);
+      if (a.post) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          sn[0][i] = sp[i];
+          sn[1][i] = sp[bp + i];
+        }
+      }
+    }
   };
 #pragma unroll
   for (int j = 0; j < NV; ++j) dyn[j].v = dnn[j].v = yn[j].v = fn[j].v = typename Vec::V(0);
-  if (b0 < b1) fetch(b0, t0);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    sn[0][i] = sn[2][i] = sn[3][i] = 0.f;
+    sn[1][i] = 1.f;
+  }
+  if (PF && b0 < b1) fetch(b0, t0);
+  ti.params(a.pre ? a.pre_w : nullptr, 0.f, pw);
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < NP; ++i) gw[j][i] = 0.f;
   bool have_gw = false;
   for (int b = b0; b < b1; ++b) {
     if (BR && (!have_gw || IG)) {
       have_gw = true;
       ti.params(a.post ? a.post_w : nullptr, 1.f, gw);
-      if (a.gate_kind) {
-        float g[NV][NP];
-        ti.params(a.gate + (IG ? (long)b * a.C : 0), 0.f, g);
+      float g[NV][NP];
+      ti.params(a.gate_kind ? a.gate + (IG ? (long)b * a.C : 0) : nullptr, 1.f, g);
+      // 0 for a channel that is not the thread's own: it then adds nothing to the sums
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int i = 0; i < NP; ++i) gw[j][i] *= g[j][i];
-      }
+        for (int i = 0; i < NP; ++i) gw[j][i] = ti.exists(j, i) ? gw[j][i] * g[j][i] : 0.f;
     }
     const float s = a.scale ? a.scale[b] : 1.0f;
     for (int t = t0; t < t1; ++t) {
+      if (!PF) fetch(b, t);
       Vec dy[NV], dn[NV], yv[NV], fv[NV];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -421,22 +458,22 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
         yv[j] = yn[j];
         fv[j] = fn[j];
       }
-      const int bn = t + 1 < t1 ? b : b + 1, tn = t + 1 < t1 ? t + 1 : t0;
-      if (bn < b1) fetch(bn, tn);
-      // statistics of the token(s); a pixel past the end has deviation 0 and adds nothing
       float mu0[NS], rs0[NS], mu1[NS], rs1[NS];
-      {
-        const long p0 = TOK ? t : ((long)t * L + ti.pl) * VEC;
-        const float* st = a.stats_in + (long)b * a.P + p0;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          const bool on = TOK || p0 + i < a.P;
-          mu0[i] = BR && a.post && on ? st[i] : 0.f;
-          rs0[i] = BR && a.post ? (on ? st[bp + i] : 0.f) : 1.f;
-          mu1[i] = a.pre && on ? st[2 * bp + i] : 0.f;
-          rs1[i] = a.pre && on ? st[3 * bp + i] : 0.f;
-        }
+      for (int i = 0; i < NS; ++i) {
+        mu0[i] = sn[0][i];
+        rs0[i] = sn[1][i];
+        mu1[i] = sn[2][i];
+        rs1[i] = sn[3][i];
       }
+      const int bn = t + 1 < t1 ? b : b + 1, tn = t + 1 < t1 ? t + 1 : t0;
+      if (PF && bn < b1) fetch(bn, tn);
+      const unsigned st = ti.start(t);
+      const int px = ti.own_pixels(t);
+      // a pixel that is not the vector's own is all zeros below, whatever stands there: it adds nothing to any sum
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+        if (!TOK && i < VEC - px) mu0[i] = rs0[i] = mu1[i] = rs1[i] = 0.f;
       float d[NV][VEC];                                        // dyt
       if (a.pre) {
         float m[2 * NS];
@@ -447,8 +484,9 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             const int q = TOK ? 0 : i, c = TOK ? i : 0;
-            const float o = dn[j].at(i), g = o * pw[j][c];
-            const float vh = (a.pre == 1 ? yv[j].at(i) - mu1[q] : yv[j].at(i)) * rs1[q];
+            const bool own = ti.mine(j, i, px);
+            const float o = own ? dn[j].at(i) : 0.f, yo = own ? yv[j].at(i) : 0.f, g = o * pw[j][c];
+            const float vh = (a.pre == 1 ? yo - mu1[q] : yo) * rs1[q];
             m[q] += g;
             m[NS + q] = fmaf(g, vh, m[NS + q]);
             acc[RN_Q_PRE_W][j][c] = fmaf(o, vh, acc[RN_Q_PRE_W][j][c]);
@@ -474,7 +512,7 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) d[j][i] = dy[j].at(i);
       }
-      ti.store(static_cast<T*>(a.dx) + ti.origin(b, a.dx_bs, t), t, d);
+      ti.store(a.dx, a.dx_bs, b, st, px, d);
       if (!BR) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -489,10 +527,10 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
             const int q = TOK ? 0 : i, c = TOK ? i : 0;
-            const float sd = ti.exists(j, i) ? d[j][i] * s : 0.f;
-            const float vh = (a.post == 1 ? fv[j].at(i) - mu0[q] : fv[j].at(i)) * rs0[q];
+            const bool own = ti.mine(j, i, px);
+            const float sd = own ? d[j][i] * s : 0.f, fo = own ? fv[j].at(i) : 0.f;
+            const float vh = (a.post == 1 ? fo - mu0[q] : fo) * rs0[q];
             img[0][j][c] = fmaf(sd, vh, img[0][j][c]);
-            // (a pixel past the end has dyt = 0: its dy is 0 and its deviation is 0)
             img[1][j][c] += sd;
             d[j][i] = sd * gw[j][c];
             m[q] += d[j][i];
@@ -514,7 +552,7 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
             }
         }
       }
-      ti.store(static_cast<T*>(a.df) + ti.origin(b, a.df_bs, t), t, d);
+      ti.store(a.df, a.df_bs, b, st, px, d);
     }
     if (IG) {
       // the image is done: its gate's gradient, and its share of the norm's parameters
@@ -559,11 +597,10 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
         if (b < a.B && ti.exists(j, i) && (TOK || ti.pl == 0)) a.part_gate[((long)b * a.S + slab) * a.C + ti.channel(j) + i] = 0.f;
   }
   if (!a.part) return;
-  // one row of partial sums per workgroup
+  // one row of partial sums per workgroup, for the quantities that are wanted
 #pragma unroll
   for (int q = 0; q < RN_Q_N; ++q) {
-    if (!BR && q < RN_Q_PRE_W) continue;
-    if (q >= RN_Q_PRE_W && !a.pre) continue;
+    if ((!BR && q < RN_Q_PRE_W) || !(a.wanted >> q & 1)) continue;
     float* out = a.part + ((long)q * a.part_rows + blockIdx.x) * a.C;
     if (TOK && L) {
       const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
@@ -579,10 +616,10 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
         }
       __syncthreads();
       for (int k = threadIdx.x; k < L * EW; k += blockDim.x) {
-        const int l = k / EW, e = k % EW, c = ((e / NP) * L + l) * VEC + e % NP;
+        const int l = k / EW, e = k % EW, c0 = ((e / NP) * L + l) * VEC, c = min(c0, a.C - VEC) + e % NP;
         float v = 0.f;
         for (int w = 0; w < waves; ++w) v += wsum[(w * L + l) * EW + e];
-        if (c < a.C) out[c] = v;
+        if (c >= c0) out[c] = v;
       }
     } else {
 #pragma unroll

@@ -105,8 +105,12 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
   const int vec = f.tok ? (dtype == JIRF_F32 ? 4 : 8) : 4;
   a.tiles = a.P;
   a.S = a.ipw = 1;
+  f.threads = 256;
   long per_block = 1;                  // workers of a workgroup
-  if (f.tok) {
+  const long image_bytes = (long)a.C * a.P * (dtype == JIRF_F32 ? 4 : 2);
+  if ((f.tok ? a.C : a.P) < vec || image_bytes >= 1l << 32) {
+    f.lanes = -1;
+  } else if (f.tok) {
     // eight channels per thread; sixteen where eight would need more than 512 threads
     const int threads8 = (a.C + 7) / 8;
     f.nv = 8 / vec;
@@ -139,7 +143,7 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
   // Workers: enough workgroups to fill the chip several times over (forward), or about twice (backward: each leaves a row
   // of partial sums per parameter).
   if (f.lanes < 0) a.tiles = (int)(((long)a.P + 63) / 64);
-  const long want = (f.lanes < 0 ? 256 : backward ? 512 : 2048) * per_block;
+  const long want = (f.lanes < 0 ? 256 : (backward ? 512 : 2048) * 256 / f.threads) * per_block;
   if (a.B >= want) {
     a.ipw = (int)((a.B + want - 1) / want);
     a.per = a.tiles;
@@ -166,7 +170,7 @@ BwdWork bwd_work(const RnArgs& a, const RnForm& f) {
   return w;
 }
 
-// Adds the partial sums up, rows in order per thread and the 32 row lanes in order, in 64 bits.  blockIdx.y 0: the branch (G1,
+// Adds the partial sums up, rows in order per thread and the row lanes in order, in 64 bits.  blockIdx.y 0: the branch (G1,
 // G0 -> dpost_w, dpost_b, dgate), 1: the norm before the next block.
 struct ReduceArgs {
   const float* part;
@@ -175,56 +179,69 @@ struct ReduceArgs {
   const float *gate, *post_w, *post_b;   // gate: null with a gate per image (its factors are in the sums already)
   int has_post, accumulate;
 };
-__device__ __forceinline__ double reduce_column(const float* part, long rows, long C, long c, double (*red)[33]) {
-  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
-  double t = 0.0;
-  if (c < C)
-    for (long r = rl; r < rows; r += 32) t += (double)part[r * C + c];
+// Sums of column c of two planes (q or r null: none) over the rows: 64 row lanes of 16 columns, eight loads in flight each.
+constexpr int RED_C = 16, RED_R = 64;
+__device__ __forceinline__ void reduce_columns(const float* q, const float* r, long rows, long C, long c, double (*red)[RED_C + 1],
+                                               double& vq, double& vr) {
+  const int cl = threadIdx.x % RED_C, rl = threadIdx.x / RED_C;
+  double tq = 0.0, tr = 0.0;
+  if (c < C) {
+    if (q)
+#pragma unroll 4
+      for (long i = rl; i < rows; i += RED_R) tq += (double)q[i * C + c];
+    if (r)
+#pragma unroll 4
+      for (long i = rl; i < rows; i += RED_R) tr += (double)r[i * C + c];
+  }
+  vq = vr = 0.0;
+  red[rl][cl] = tq;
   __syncthreads();
-  red[rl][cl] = t;
-  __syncthreads();
-  double v = 0.0;
   if (rl == 0)
-#pragma unroll
-    for (int r = 0; r < 32; ++r) v += red[r][cl];
-  return v;
+#pragma unroll 8
+    for (int i = 0; i < RED_R; ++i) vq += red[i][cl];
+  if (!r) return;                       // (the same for every thread)
+  __syncthreads();
+  red[rl][cl] = tr;
+  __syncthreads();
+  if (rl == 0)
+#pragma unroll 8
+    for (int i = 0; i < RED_R; ++i) vr += red[i][cl];
 }
 __device__ __forceinline__ void reduce_out(float* out, long c, double v, int accumulate) {
   if (out) out[c] = accumulate ? (float)((double)out[c] + v) : (float)v;
 }
-__global__ __launch_bounds__(1024) void rn_reduce(const ReduceArgs a) {
-  __shared__ double red[32][33];
-  const long c = (long)blockIdx.x * 32 + (threadIdx.x & 31);
-  const bool writer = threadIdx.x < 32 && c < a.C;
+__global__ __launch_bounds__(RED_C * RED_R) void rn_reduce(const ReduceArgs a) {
+  __shared__ double red[RED_R][RED_C + 1];
+  const long c = (long)blockIdx.x * RED_C + threadIdx.x % RED_C;
+  const bool writer = threadIdx.x < RED_C && c < a.C;
   const long plane = a.rows * a.C;
+  double v0, v1;
   if (blockIdx.y == 0) {
     if (!a.dpost_w && !a.dpost_b && !a.dgate) return;
-    const double g1 = reduce_column(a.part + RN_Q_G1 * plane, a.rows, a.C, c, red);
-    const bool g0_used = a.dpost_b || (a.dgate && a.post_b);
-    const double g0 = g0_used ? reduce_column(a.part + RN_Q_G0 * plane, a.rows, a.C, c, red) : 0.0;
+    const bool g1_used = a.dpost_w || a.dgate, g0_used = a.dpost_b || (a.dgate && a.post_b);
+    reduce_columns(g1_used ? a.part + RN_Q_G1 * plane : nullptr, g0_used ? a.part + RN_Q_G0 * plane : nullptr, a.rows, a.C, c, red, v0, v1);
     if (!writer) return;
     const double g = a.gate ? (double)a.gate[c] : 1.0;
-    reduce_out(a.dpost_w, c, g * g1, a.accumulate);
-    reduce_out(a.dpost_b, c, g * g0, a.accumulate);
-    reduce_out(a.dgate, c, a.has_post ? a.post_w[c] * g1 + (a.post_b ? a.post_b[c] * g0 : 0.0) : g1, a.accumulate);
+    reduce_out(a.dpost_w, c, g * v0, a.accumulate);
+    reduce_out(a.dpost_b, c, g * v1, a.accumulate);
+    reduce_out(a.dgate, c, a.has_post ? a.post_w[c] * v0 + (a.post_b ? a.post_b[c] * v1 : 0.0) : v0, a.accumulate);
   } else {
-    if (a.dpre_w) {
-      const double v = reduce_column(a.part + RN_Q_PRE_W * plane, a.rows, a.C, c, red);
-      if (writer) reduce_out(a.dpre_w, c, v, a.accumulate);
-    }
-    if (a.dpre_b) {
-      const double v = reduce_column(a.part + RN_Q_PRE_B * plane, a.rows, a.C, c, red);
-      if (writer) reduce_out(a.dpre_b, c, v, a.accumulate);
-    }
+    if (!a.dpre_w && !a.dpre_b) return;
+    reduce_columns(a.dpre_w ? a.part + RN_Q_PRE_W * plane : nullptr, a.dpre_b ? a.part + RN_Q_PRE_B * plane : nullptr, a.rows, a.C, c, red,
+                   v0, v1);
+    if (!writer) return;
+    reduce_out(a.dpre_w, c, v0, a.accumulate);
+    reduce_out(a.dpre_b, c, v1, a.accumulate);
   }
 }
 // dgate [B][C] from the [B][S][C] sums of a gate per image
-__global__ __launch_bounds__(1024) void rn_reduce_gate(const float* __restrict__ part, long S, long C, float* __restrict__ dgate,
-                                                       int accumulate) {
-  __shared__ double red[32][33];
-  const long c = (long)blockIdx.x * 32 + (threadIdx.x & 31);
-  const double v = reduce_column(part + (long)blockIdx.y * S * C, S, C, c, red);
-  if (threadIdx.x < 32 && c < C) reduce_out(dgate + (long)blockIdx.y * C, c, v, accumulate);
+__global__ __launch_bounds__(RED_C * RED_R) void rn_reduce_gate(const float* __restrict__ part, long S, long C,
+                                                                float* __restrict__ dgate, int accumulate) {
+  __shared__ double red[RED_R][RED_C + 1];
+  const long c = (long)blockIdx.x * RED_C + threadIdx.x % RED_C;
+  double v, none;
+  reduce_columns(part + (long)blockIdx.y * S * C, nullptr, S, C, c, red, v, none);
+  if (threadIdx.x < RED_C && c < C) reduce_out(dgate + (long)blockIdx.y * C, c, v, accumulate);
 }
 
 }  // namespace
@@ -327,6 +344,9 @@ int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, lon
       a.part_gate = dgate ? work + wk.rowsum + wk.part : nullptr;
     }
     a.dgate = gate_kind == 2 ? dgate : nullptr;
+    const bool gate1 = gate_kind == 1 && dgate;
+    a.wanted = (dpost_w || gate1 ? 1 << RN_Q_G1 : 0) | (dpost_b || (gate1 && post_kind == 1 && post_b) ? 1 << RN_Q_G0 : 0) |
+               (dpre_w ? 1 << RN_Q_PRE_W : 0) | (dpre_b ? 1 << RN_Q_PRE_B : 0);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int reads = 1 + (pre_kind ? 2 : 0) + (branch ? 1 : 0);
     const int mode = !branch ? RN_BWD_STREAM : gate_kind == 2 ? RN_BWD_IMAGE_GATE : RN_BWD_BRANCH;
@@ -337,9 +357,9 @@ int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, lon
     if (params) {
       const ReduceArgs r{a.part, a.part_rows, C, dpost_w, dpost_b, gate_kind == 1 ? dgate : nullptr, dpre_w, dpre_b,
                          gate_kind == 1 ? gate : nullptr, post_w, post_kind == 1 ? post_b : nullptr, post_kind, accumulate};
-      hipLaunchKernelGGL(rn_reduce, dim3((unsigned)((C + 31) / 32), 2), dim3(1024), 0, s, r);
+      hipLaunchKernelGGL(rn_reduce, dim3((unsigned)((C + RED_C - 1) / RED_C), 2), dim3(RED_C * RED_R), 0, s, r);
       if (gate_kind == 2 && dgate && a.S > 1)
-        hipLaunchKernelGGL(rn_reduce_gate, dim3((unsigned)((C + 31) / 32), (unsigned)B), dim3(1024), 0, s, a.part_gate, (long)a.S,
+        hipLaunchKernelGGL(rn_reduce_gate, dim3((unsigned)((C + RED_C - 1) / RED_C), (unsigned)B), dim3(RED_C * RED_R), 0, s, a.part_gate, (long)a.S,
                            (long)C, dgate, accumulate);
     }
     JIRF_HIP_CHECK(hipGetLastError());
