@@ -45,6 +45,16 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
+// A chunk's addresses come out of memory: said to be device memory here, or every access would take the slower flat path.
+template <typename P>
+__device__ __forceinline__ const __attribute__((address_space(1))) P* dev(const void* p, size_t byte) {
+  return reinterpret_cast<const __attribute__((address_space(1))) P*>(reinterpret_cast<uintptr_t>(p) + byte);
+}
+template <typename P>
+__device__ __forceinline__ __attribute__((address_space(1))) P* dev(void* p, size_t byte) {
+  return reinterpret_cast<__attribute__((address_space(1))) P*>(reinterpret_cast<uintptr_t>(p) + byte);
+}
+
 template <int TY>
 struct Raw {              // eight elements as loaded
   u32x4 a, b;             // b: fp32 only
@@ -53,11 +63,10 @@ template <int TY>
 __device__ __forceinline__ Raw<TY> clip_load8(const void* p, unsigned g) {
   Raw<TY> r{};
   if constexpr (TY == TY_F32) {
-    const u32x4_a4* q = reinterpret_cast<const u32x4_a4*>(static_cast<const float*>(p) + (size_t)g * CLIP_E);
-    r.a = q[0];
-    r.b = q[1];
+    r.a = *dev<u32x4_a4>(p, g * 32u);
+    r.b = *dev<u32x4_a4>(p, g * 32u + 16u);
   } else {
-    r.a = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(p) + (size_t)g * CLIP_E);
+    r.a = *dev<u32x4_a2>(p, g * 16u);
   }
   return r;
 }
@@ -87,38 +96,37 @@ __device__ __forceinline__ f32x8 clip_widen(const Raw<TY>& r) {
 template <int TY>
 __device__ __forceinline__ void clip_store8(void* p, unsigned g, const f32x8& v) {
   if constexpr (TY == TY_F32) {
-    u32x4_a4* q = reinterpret_cast<u32x4_a4*>(static_cast<float*>(p) + (size_t)g * CLIP_E);
     u32x4 a, b;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       a[i] = __float_as_uint(v[i]);
       b[i] = __float_as_uint(v[4 + i]);
     }
-    q[0] = a;
-    q[1] = b;
+    *dev<u32x4_a4>(p, g * 32u) = a;
+    *dev<u32x4_a4>(p, g * 32u + 16u) = b;
   } else if constexpr (TY == TY_BF16) {
     bf16x8 h;
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = (__bf16)v[i];
-    *reinterpret_cast<u32x4_a2*>(static_cast<uint16_t*>(p) + (size_t)g * CLIP_E) = __builtin_bit_cast(u32x4, h);
+    *dev<u32x4_a2>(p, g * 16u) = __builtin_bit_cast(u32x4, h);
   } else {
     f16x8 h;
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i];
-    *reinterpret_cast<u32x4_a2*>(static_cast<uint16_t*>(p) + (size_t)g * CLIP_E) = __builtin_bit_cast(u32x4, h);
+    *dev<u32x4_a2>(p, g * 16u) = __builtin_bit_cast(u32x4, h);
   }
 }
 template <int TY>
 __device__ __forceinline__ float clip_load1(const void* p, unsigned i) {
-  if constexpr (TY == TY_F32) return static_cast<const float*>(p)[i];
-  else if constexpr (TY == TY_BF16) return __uint_as_float((unsigned)static_cast<const uint16_t*>(p)[i] << 16);
-  else return (float)static_cast<const _Float16*>(p)[i];
+  if constexpr (TY == TY_F32) return *dev<float>(p, i * 4u);
+  else if constexpr (TY == TY_BF16) return __uint_as_float((unsigned)*dev<uint16_t>(p, i * 2u) << 16);
+  else return (float)*dev<_Float16>(p, i * 2u);
 }
 template <int TY>
 __device__ __forceinline__ void clip_store1(void* p, unsigned i, float v) {
-  if constexpr (TY == TY_F32) static_cast<float*>(p)[i] = v;
-  else if constexpr (TY == TY_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
-  else static_cast<_Float16*>(p)[i] = (_Float16)v;
+  if constexpr (TY == TY_F32) *dev<float>(p, i * 4u) = v;
+  else if constexpr (TY == TY_BF16) *dev<__bf16>(p, i * 2u) = (__bf16)v;
+  else *dev<_Float16>(p, i * 2u) = (_Float16)v;
 }
 // A maximum that a NaN wins: the bit patterns of |v| order like the values, with every NaN above infinity.
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -234,7 +242,12 @@ __global__ __launch_bounds__(CLIP_T) void norm_kernel(const ClipChunk* __restric
                                                       double* __restrict__ part) {
   __shared__ double red[CLIP_T / 64];
   ClipAcc acc;
-  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) norm_any<MAX>(chunks[c], threadIdx.x, acc);
+  ClipChunk next = chunks[blockIdx.x];     // (a list with a workgroup has a chunk for it)
+  for (int c = blockIdx.x; c < n_chunks; c += gridDim.x) {
+    const ClipChunk ck = next;
+    if (c + (int)gridDim.x < n_chunks) next = chunks[c + gridDim.x];
+    norm_any<MAX>(ck, threadIdx.x, acc);
+  }
   const double r = block_combine<MAX, CLIP_T>(MAX ? (double)__uint_as_float(acc.mx) : acc.sum, red);
   if (threadIdx.x == 0) part[blockIdx.x] = r;
 }
@@ -252,25 +265,92 @@ __global__ __launch_bounds__(CLIP_T) void clip_kernel(const ClipChunk* __restric
   for (int c = n_chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) scale_any(chunks[c], threadIdx.x, k);
 }
 
-// Few chunks: one workgroup of four chunk teams does both passes in one launch.
-constexpr int CLIP_SMALL_T = 1024, CLIP_SMALL_CHUNKS = 32;
+// Small lists (at most CLIP_SMALL_E elements in CLIP_SMALL_CHUNKS chunks of CLIP_SMALL_T): one workgroup, one launch.  Teams
+// of two waves hold up to eight chunks each in registers between the norm and the store, so memory is waited for once.
+constexpr int CLIP_SMALL_T = 128, CLIP_SMALL_TEAMS = 8, CLIP_SMALL_U = 8;
+constexpr int CLIP_SMALL_CHUNK = CLIP_SMALL_T * CLIP_E, CLIP_SMALL_CHUNKS = CLIP_SMALL_TEAMS * CLIP_SMALL_U;
+constexpr long CLIP_SMALL_E = (long)CLIP_SMALL_CHUNK * CLIP_SMALL_CHUNKS;
 template <bool MAX>
-__global__ __launch_bounds__(CLIP_SMALL_T) void norm_clip_kernel(const ClipChunk* __restrict__ chunks, int n_chunks, int writes,
-                                                                 double max_norm, double grad_scale, double* __restrict__ stats) {
-  __shared__ double red[CLIP_SMALL_T / 64];
-  const unsigned team = threadIdx.x / CLIP_T, t = threadIdx.x % CLIP_T;
+__global__ __launch_bounds__(CLIP_SMALL_T * CLIP_SMALL_TEAMS) void norm_clip_kernel(const ClipChunk* __restrict__ chunks, int n_chunks,
+                                                                                    int writes, double max_norm, double grad_scale,
+                                                                                    double* __restrict__ stats) {
+  __shared__ double red[CLIP_SMALL_T * CLIP_SMALL_TEAMS / 64];
+  const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / CLIP_SMALL_T);     // (whole waves)
+  const unsigned t = threadIdx.x % CLIP_SMALL_T;
+  ClipChunk ck[CLIP_SMALL_U];
+#pragma unroll
+  for (int u = 0; u < CLIP_SMALL_U; ++u) {
+    ck[u] = chunks[min(team + u * CLIP_SMALL_TEAMS, n_chunks - 1)];
+    if (team + u * CLIP_SMALL_TEAMS >= n_chunks) ck[u].n = 0;
+  }
+  // groups of eight, and the few elements past the last whole group; every load is issued before the first is used
+  u32x4 ra[CLIP_SMALL_U], rb[CLIP_SMALL_U];
+  unsigned rt[CLIP_SMALL_U];
+#pragma unroll
+  for (int u = 0; u < CLIP_SMALL_U; ++u) {
+    ra[u] = rb[u] = u32x4(0u);
+    rt[u] = 0u;
+    const unsigned wide = (ck[u].types & 0xff) == TY_F32 ? 1u : 0u, groups = ck[u].n / CLIP_E, i = groups * CLIP_E + t;
+    if (t < groups) {
+      ra[u] = *dev<u32x4_a2>(ck[u].src, t * 16u << wide);
+      if (wide) rb[u] = *dev<u32x4_a2>(ck[u].src, t * 32u + 16u);
+    }
+    if (i < ck[u].n) {
+      if (wide) rt[u] = *dev<unsigned>(ck[u].src, i * 4u);
+      else rt[u] = *dev<uint16_t>(ck[u].src, i * 2u);
+    }
+  }
+  f32x8 v[CLIP_SMALL_U];
+  float tail[CLIP_SMALL_U];
+#pragma unroll
+  for (int u = 0; u < CLIP_SMALL_U; ++u) {
+    const unsigned ty = ck[u].types & 0xff;
+    if (ty == TY_F32) {
+      v[u] = clip_widen<TY_F32>(Raw<TY_F32>{ra[u], rb[u]});
+      tail[u] = __uint_as_float(rt[u]);
+    } else if (ty == TY_BF16) {
+      v[u] = clip_widen<TY_BF16>(Raw<TY_BF16>{ra[u], rb[u]});
+      tail[u] = __uint_as_float(rt[u] << 16);
+    } else {
+      v[u] = clip_widen<TY_F16>(Raw<TY_F16>{ra[u], rb[u]});
+      tail[u] = (float)__builtin_bit_cast(_Float16, (uint16_t)rt[u]);
+    }
+  }
   ClipAcc acc;
-  for (int c = team; c < n_chunks; c += CLIP_SMALL_T / CLIP_T) norm_any<MAX>(chunks[c], t, acc);
-  const double raw = block_combine<MAX, CLIP_SMALL_T>(MAX ? (double)__uint_as_float(acc.mx) : acc.sum, red);
+#pragma unroll
+  for (int u = 0; u < CLIP_SMALL_U; ++u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (MAX) acc.mx = max(acc.mx, abs_bits(v[u][i]));
+      else acc.sum = fma((double)v[u][i], (double)v[u][i], acc.sum);
+    }
+    if (MAX) acc.mx = max(acc.mx, abs_bits(tail[u]));
+    else acc.sum = fma((double)tail[u], (double)tail[u], acc.sum);
+  }
+  const double raw =
+      block_combine<MAX, CLIP_SMALL_T * CLIP_SMALL_TEAMS>(MAX ? (double)__uint_as_float(acc.mx) : acc.sum, red);
   const float k = clip_factor<MAX>(raw, max_norm, grad_scale, stats, threadIdx.x == 0);
-  if (writes)
-    for (int c = team; c < n_chunks; c += CLIP_SMALL_T / CLIP_T) scale_any(chunks[c], t, k);
+  if (!writes) return;
+#pragma unroll
+  for (int u = 0; u < CLIP_SMALL_U; ++u) {
+    const unsigned td = ck[u].types >> 8, groups = ck[u].n / CLIP_E, i = groups * CLIP_E + t;
+    if (t < groups) {
+      if (td == TY_F32) clip_store8<TY_F32>(ck[u].dst, t, v[u] * k);
+      else if (td == TY_BF16) clip_store8<TY_BF16>(ck[u].dst, t, v[u] * k);
+      else clip_store8<TY_F16>(ck[u].dst, t, v[u] * k);
+    }
+    if (i < ck[u].n) {
+      if (td == TY_F32) clip_store1<TY_F32>(ck[u].dst, i, tail[u] * k);
+      else if (td == TY_BF16) clip_store1<TY_BF16>(ck[u].dst, i, tail[u] * k);
+      else clip_store1<TY_F16>(ck[u].dst, i, tail[u] * k);
+    }
+  }
 }
 
 struct ClipPlan {
   int device = 0;
   int n_chunks = 0, blocks = 1;
-  bool writes = false;
+  bool writes = false, small = false;
   double bytes_read = 0.0, bytes_written = 0.0;
   long total = 0;
   DeviceBuffer chunks;
@@ -354,9 +434,14 @@ int jirf_train_grad_clip_plan_create(int n, const void* const* src, const int* s
     }
     if (dst) check_ranges(n, src, src_dtype, dst, dst_dtype, count);
     auto plan = std::make_unique<ClipPlan>();
-    // enough chunks to occupy every workgroup, at least one step of a workgroup each, at most 64 Ki elements
-    const long step = CLIP_T * CLIP_E;
-    const long chunk = std::min<long>(65536, std::max<long>(step, (total / CLIP_MAX_BLOCKS + step - 1) / step * step));
+    // one workgroup takes a small list whole
+    long small_chunks = 0;
+    for (int i = 0; i < n && small_chunks <= CLIP_SMALL_CHUNKS; ++i) small_chunks += (count[i] + CLIP_SMALL_CHUNK - 1) / CLIP_SMALL_CHUNK;
+    plan->small = small_chunks <= CLIP_SMALL_CHUNKS;
+    // else about four chunks for every workgroup, of whole steps of CLIP_U accesses in flight (8 Ki elements), at most 64 Ki
+    const long step = CLIP_T * CLIP_E * CLIP_U;
+    const long chunk = plan->small ? CLIP_SMALL_CHUNK
+                                   : std::min<long>(65536, std::max<long>(step, (total / (4 * CLIP_MAX_BLOCKS) + step - 1) / step * step));
     std::vector<ClipChunk> chunks;
     for (int i = 0; i < n; ++i) {
       const int ts = type_of(src_dtype[i]), td = dst ? type_of(dst_dtype[i]) : TY_F32;
@@ -367,29 +452,32 @@ int jirf_train_grad_clip_plan_create(int n, const void* const* src, const int* s
       plan->bytes_read += (double)count[i] * type_bytes(ts);
       if (dst) plan->bytes_written += (double)count[i] * type_bytes(td);
     }
+    if (chunks.empty()) chunks.push_back({nullptr, nullptr, 0, 0});      // nothing to read, but a row for the kernel
     JIRF_REQUIRE(chunks.size() < (size_t)1 << 30, JIRF_EINVAL, "grad_clip_plan_create: too many elements");
     JIRF_HIP_CHECK(hipGetDevice(&plan->device));
     plan->total = total;
     plan->writes = dst != nullptr;
     plan->n_chunks = (int)chunks.size();
-    plan->blocks = std::max(1, std::min(CLIP_MAX_BLOCKS, plan->n_chunks));
-    if (!chunks.empty()) {
-      plan->chunks.ensure(chunks.size() * sizeof(ClipChunk));
-      JIRF_HIP_CHECK(hipMemcpy(plan->chunks.p, chunks.data(), chunks.size() * sizeof(ClipChunk), hipMemcpyHostToDevice));
-    }
+    // the same number of chunks for every workgroup, but the last few
+    const int rounds = std::max(1, (plan->n_chunks + CLIP_MAX_BLOCKS - 1) / CLIP_MAX_BLOCKS);
+    plan->blocks = std::max(1, (plan->n_chunks + rounds - 1) / rounds);
+    plan->chunks.ensure(chunks.size() * sizeof(ClipChunk));
+    JIRF_HIP_CHECK(hipMemcpy(plan->chunks.p, chunks.data(), chunks.size() * sizeof(ClipChunk), hipMemcpyHostToDevice));
     *plan_out = plan.release();
     return JIRF_OK;
   });
 }
 
 long jirf_train_grad_clip_work_doubles(const void* plan) {
-  return plan ? static_cast<const ClipPlan*>(plan)->blocks : -1;
+  if (!plan) return -1;
+  const ClipPlan* pl = static_cast<const ClipPlan*>(plan);
+  return pl->small ? 0 : pl->blocks;
 }
 
 int jirf_train_grad_clip_run(const void* plan, int norm_kind, double max_norm, double grad_scale, double* stats, double* work,
                              void* stream) {
   return guarded_c([&] {
-    JIRF_REQUIRE(plan && stats && work, JIRF_EINVAL, "grad_clip_run: null argument");
+    JIRF_REQUIRE(plan && stats && (work || static_cast<const ClipPlan*>(plan)->small), JIRF_EINVAL, "grad_clip_run: null argument");
     JIRF_REQUIRE(norm_kind == JIRF_NORM_L2 || norm_kind == JIRF_NORM_MAX, JIRF_EINVAL, "grad_clip_run: norm_kind %d", norm_kind);
     JIRF_REQUIRE(grad_scale > 0.0 && std::isfinite(grad_scale) && !std::isnan(max_norm), JIRF_EINVAL,
                  "grad_clip_run: grad_scale must be positive and finite, max_norm a number");
@@ -400,9 +488,9 @@ int jirf_train_grad_clip_run(const void* plan, int norm_kind, double max_norm, d
     hipStream_t s = static_cast<hipStream_t>(stream);
     const ClipChunk* ck = static_cast<const ClipChunk*>(pl->chunks.p);
     const bool mx = norm_kind == JIRF_NORM_MAX;
-    if (pl->n_chunks <= CLIP_SMALL_CHUNKS) {
+    if (pl->small) {
       Scope sc("train_grad_norm_clip", 3.0 * pl->total, pl->bytes_read + pl->bytes_written, s);
-      hipLaunchKernelGGL(mx ? norm_clip_kernel<true> : norm_clip_kernel<false>, dim3(1), dim3(CLIP_SMALL_T), 0, s, ck, pl->n_chunks,
+      hipLaunchKernelGGL(mx ? norm_clip_kernel<true> : norm_clip_kernel<false>, dim3(1), dim3(CLIP_SMALL_T * CLIP_SMALL_TEAMS), 0, s, ck, pl->n_chunks,
                          pl->writes ? 1 : 0, max_norm, grad_scale, stats);
       JIRF_HIP_CHECK(hipGetLastError());
       return JIRF_OK;

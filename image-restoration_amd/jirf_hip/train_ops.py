@@ -10,6 +10,7 @@ any.  There is no CPU path and no autograd graph: the backward is called by name
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -20,6 +21,9 @@ from jirf_hip import check, lib
 LAYOUTS = {"planar": 0, "tokens": 1}
 NORM_KINDS = {"WithBias": 1, "BiasFree": 2, "RMS": 3, 1: 1, 2: 2, 3: 3}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 4, torch.float16: 5}
+# the current stream's handle without the stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
 Norm = Tuple[object, torch.Tensor, Optional[torch.Tensor]]
 
 
@@ -36,19 +40,19 @@ def _sizes(x: torch.Tensor, layout: str):
         raise ValueError("residual_norm needs GPU tensors: there is no CPU path")
     if x.dtype not in _DTYPES:
         raise ValueError(f"dtype {x.dtype}: only float32, bfloat16 and float16")
-    if x.dim() < 3 or (layout == "tokens" and x.dim() != 3):
-        raise ValueError(f"{layout} activations are [B, C, ...] / [B, P, C], got shape {tuple(x.shape)}")
-    if x.numel() == 0:
-        raise ValueError(f"empty activation {tuple(x.shape)}")
+    shape, n = x.shape, x.numel()
+    if len(shape) < 3 or (layout == "tokens" and len(shape) != 3):
+        raise ValueError(f"{layout} activations are [B, C, ...] / [B, P, C], got shape {tuple(shape)}")
+    if n == 0:
+        raise ValueError(f"empty activation {tuple(shape)}")
     if layout == "planar":
-        B, Cn = x.shape[0], x.shape[1]
-        return B, Cn, x.numel() // (B * Cn)
-    return x.shape[0], x.shape[2], x.shape[1]
+        return shape[0], shape[1], n // (shape[0] * shape[1])
+    return shape[0], shape[2], shape[1]
 
 
 def _bs(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
     """Batch stride (0: dense) of an activation that has to match `like`."""
-    if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    if t is not like and (t.shape != like.shape or t.dtype != like.dtype or t.get_device() != like.get_device()):
         raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(like.shape)} {like.dtype} on {like.device}")
     if t.is_contiguous():
         return 0
@@ -58,7 +62,7 @@ def _bs(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
 
 
 def _param(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> int:
-    if tuple(t.shape) != shape or t.dtype != torch.float32 or t.device != like.device or not t.is_contiguous():
+    if t.shape != shape or t.dtype != torch.float32 or t.get_device() != like.get_device() or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous float32 tensor {shape} on {like.device} is needed, got {tuple(t.shape)} {t.dtype} "
                          f"on {t.device}")
     return t.data_ptr()
@@ -85,10 +89,22 @@ def _gate(gate: Optional[torch.Tensor], B: int, Cn: int, like: torch.Tensor):
     return 2, _param("gate", gate, (B, Cn), like)
 
 
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _on_device(fn):
+    """Runs fn with the device of its first tensor argument current (a switch only where it is not already)."""
+    def call(*args, **kw):
+        t = next((a for a in (*args, *kw.values()) if isinstance(a, torch.Tensor)), None)
+        if t is None or not t.is_cuda or t.get_device() == torch.cuda.current_device():
+            return fn(*args, **kw)
+        with torch.cuda.device(t.device):
+            return fn(*args, **kw)
+    return functools.wraps(fn)(call)
 
 
+def _new(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
+@_on_device
 def residual_norm(x: torch.Tensor, branch: torch.Tensor, *, post: Optional[Norm] = None, gate: Optional[torch.Tensor] = None,
                   scale: Optional[torch.Tensor] = None, pre: Optional[Norm] = None, layout: str = "planar", eps: float = 1e-5,
                   save_stats: bool = False, out: Optional[torch.Tensor] = None,
@@ -108,18 +124,18 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, *, post: Optional[Norm]
     sp = None if scale is None else _param("scale", scale, (B,), x)
     if norm_out is not None and not k1:
         raise ValueError("norm_out without a pre norm")
-    dev = x.device
-    with torch.cuda.device(dev):
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev) if out is None else out
-        n = (torch.empty(x.shape, dtype=x.dtype, device=dev) if norm_out is None else norm_out) if k1 else None
-        stats = torch.empty((4, B, P), dtype=torch.float32, device=dev) if save_stats else None
-        check(lib().jirf_train_residual_norm(
-            x.data_ptr(), _bs("x", x, x), branch.data_ptr(), fb, _DTYPES[x.dtype], LAYOUTS[layout], k0, w0, b0, gk, gp, sp, k1, w1,
-            b1, eps, y.data_ptr(), 0 if out is None else _bs("out", y, x), n.data_ptr() if k1 else None,
-            0 if norm_out is None else _bs("norm_out", n, x), stats.data_ptr() if save_stats else None, B, Cn, P, _stream(dev)))
+    y = _new(x) if out is None else out
+    n = (_new(x) if norm_out is None else norm_out) if k1 else None
+    stats = x.new_empty((4, B, P), dtype=torch.float32) if save_stats else None
+    check(lib().jirf_train_residual_norm(
+        x.data_ptr(), _bs("x", x, x), branch.data_ptr(), fb, _DTYPES[x.dtype], LAYOUTS[layout], k0, w0, b0, gk, gp, sp, k1, w1,
+        b1, eps, y.data_ptr(), 0 if out is None else _bs("out", y, x), n.data_ptr() if k1 else None,
+        0 if norm_out is None else _bs("norm_out", n, x), stats.data_ptr() if save_stats else None, B, Cn, P,
+        _raw_stream(x.get_device())))
     return ResidualNorm(y, n, stats)
 
 
+@_on_device
 def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y: Optional[torch.Tensor],
                       branch: Optional[torch.Tensor], stats: Optional[torch.Tensor], *, post: Optional[Norm] = None,
                       gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, pre: Optional[Norm] = None,
@@ -137,31 +153,35 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
     sp = None if scale is None else _param("scale", scale, (B,), like)
     if k1 and (dn is None or y is None):
         raise ValueError("residual_norm_bwd: the pre norm needs dn and y")
-    if (k0 or gk) and branch is None:
+    use_f = k0 or gk
+    if use_f and branch is None:
         raise ValueError("residual_norm_bwd: a post norm or gate needs the branch")
     if (k0 or k1) and stats is None:
         raise ValueError("residual_norm_bwd: a norm needs the forward's stats (save_stats=True)")
-    st = None if not (k0 or k1) else _param("stats", stats, (4, B, P), like)
-    use_f = bool(k0 or gk)
-    dev = like.device
+    if dy is None and not k1:
+        raise ValueError("residual_norm_bwd: without a pre norm dy is needed")
+    st = _param("stats", stats, (4, B, P), like) if k0 or k1 else None
+    dtype, lay = _DTYPES[like.dtype], LAYOUTS[layout]
     L = lib()
-    with torch.cuda.device(dev):
-        dx = torch.empty(like.shape, dtype=like.dtype, device=dev)
-        df = torch.empty(like.shape, dtype=like.dtype, device=dev)
-        # one allocation for the parameter gradients and the workspace
-        new = lambda *s: torch.empty(s, dtype=torch.float32, device=dev)     # noqa: E731
-        dgate = None if gk == 0 else (new(Cn) if gk == 1 else new(B, Cn))
-        dpost_w, dpost_b = new(Cn) if k0 else None, new(Cn) if b0 is not None else None
-        dpre_w, dpre_b = new(Cn) if k1 else None, new(Cn) if b1 is not None else None
-        work = new(max(1, L.jirf_train_residual_norm_bwd_work_floats(_DTYPES[like.dtype], LAYOUTS[layout], k0, gk, k1, B, Cn, P)))
-        ptr = lambda t: None if t is None else t.data_ptr()                  # noqa: E731
-        check(L.jirf_train_residual_norm_bwd(
-            ptr(dy), 0 if dy is None else _bs("dy", dy, like), ptr(dn) if k1 else None, _bs("dn", dn, like) if k1 else 0,
-            ptr(y) if k1 else None, _bs("y", y, like) if k1 else 0, ptr(branch) if use_f else None,
-            _bs("branch", branch, like) if use_f else 0, st, _DTYPES[like.dtype], LAYOUTS[layout], k0, w0, b0, gk, gp, sp, k1, w1,
-            dx.data_ptr(), 0, df.data_ptr(), 0, ptr(dpost_w), ptr(dpost_b), ptr(dgate), ptr(dpre_w), ptr(dpre_b), 0,
-            work.data_ptr(), B, Cn, P, _stream(dev)))
-    return dict(dx=dx, dbranch=df, dgate=dgate, dpost_w=dpost_w, dpost_b=dpost_b, dpre_w=dpre_w, dpre_b=dpre_b)
+    dx, df = _new(like), _new(like)
+    # the [C] gradients are rows of one tensor
+    rows = [None] * 5
+    wanted = [i for i, on in enumerate((k0, b0 is not None, gk == 1, k1, b1 is not None)) if on]
+    if wanted:
+        for i, t in zip(wanted, like.new_empty((len(wanted), Cn), dtype=torch.float32).unbind()):
+            rows[i] = t
+    if gk == 2:
+        rows[2] = like.new_empty((B, Cn), dtype=torch.float32)
+    need = L.jirf_train_residual_norm_bwd_work_floats(dtype, lay, k0, gk, k1, B, Cn, P)
+    work = like.new_empty(max(1, need), dtype=torch.float32)
+    p = [None if t is None else t.data_ptr() for t in rows]
+    check(L.jirf_train_residual_norm_bwd(
+        None if dy is None else dy.data_ptr(), 0 if dy is None else _bs("dy", dy, like), dn.data_ptr() if k1 else None,
+        _bs("dn", dn, like) if k1 else 0, y.data_ptr() if k1 else None, _bs("y", y, like) if k1 else 0,
+        branch.data_ptr() if use_f else None, _bs("branch", branch, like) if use_f else 0, st, dtype, lay, k0, w0, b0, gk, gp, sp,
+        k1, w1, dx.data_ptr(), 0, df.data_ptr(), 0, p[0], p[1], p[2], p[3], p[4], 0, work.data_ptr(), B, Cn, P,
+        _raw_stream(like.get_device())))
+    return dict(dx=dx, dbranch=df, dgate=rows[2], dpost_w=rows[0], dpost_b=rows[1], dpre_w=rows[3], dpre_b=rows[4])
 
 
 class GradientClip:
@@ -208,12 +228,15 @@ class GradientClip:
         grad_scale * min(max_norm / (norm + 1e-6), 1) (max_norm <= 0: grad_scale).  norm: 2 or math.inf."""
         if norm not in (2, math.inf):
             raise ValueError(f"GradientClip: norm {norm}: 2 or inf")
-        with torch.cuda.device(self.device):
-            stats = torch.empty(3 + self._work, dtype=torch.float64, device=self.device)
-            p = stats.data_ptr()
-            check(self._lib.jirf_train_grad_clip_run(self._plan, 0 if norm == 2 else 1, max_norm, grad_scale, p, p + 24,
-                                                     _stream(self.device)))
-        return stats[:3]
+        index = self.device.index
+        if index != torch.cuda.current_device():
+            with torch.cuda.device(self.device):
+                return self.run(max_norm, norm=norm, grad_scale=grad_scale)
+        stats = torch.empty(3 + self._work, dtype=torch.float64, device=self.device)
+        p = stats.data_ptr()
+        check(self._lib.jirf_train_grad_clip_run(self._plan, 0 if norm == 2 else 1, max_norm, grad_scale, p,
+                                                 p + 24 if self._work else None, _raw_stream(index)))
+        return stats[:3] if self._work else stats
 
     def __del__(self):
         if getattr(self, "_plan", None) is not None:
