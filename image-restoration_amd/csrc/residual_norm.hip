@@ -171,41 +171,54 @@ BwdWork bwd_work(const RnArgs& a, const RnForm& f) {
 }
 
 // Adds the partial sums up, rows in order per thread and the row lanes in order, in 64 bits.  blockIdx.y 0: the branch (G1,
-// G0 -> dpost_w, dpost_b, dgate), 1: the norm before the next block.
+// G0 -> dpost_w, dpost_b, dgate), 1: the norm before the next block, 2 + b: image b's gate from its S workers.
 struct ReduceArgs {
   const float* part;
   long rows, C;
   float *dpost_w, *dpost_b, *dgate, *dpre_w, *dpre_b;
   const float *gate, *post_w, *post_b;   // gate: null with a gate per image (its factors are in the sums already)
   int has_post, accumulate;
+  const float* part_gate;                // [B][S][C], for dgate_image [B][C]
+  float* dgate_image;
+  long S;
 };
-// Sums of column c of two planes (q or r null: none) over the rows: 64 row lanes of 16 columns, eight loads in flight each.
+// Sums of column c of two planes (r null: none) over the rows: 64 row lanes of 16 columns, eight loads of each in flight.
 constexpr int RED_C = 16, RED_R = 64;
+template <bool TWO>
 __device__ __forceinline__ void reduce_columns(const float* q, const float* r, long rows, long C, long c, double (*red)[RED_C + 1],
                                                double& vq, double& vr) {
   const int cl = threadIdx.x % RED_C, rl = threadIdx.x / RED_C;
-  double tq = 0.0, tr = 0.0;
+  double t[2] = {0.0, 0.0};
   if (c < C) {
-    if (q)
-#pragma unroll 4
-      for (long i = rl; i < rows; i += RED_R) tq += (double)q[i * C + c];
-    if (r)
-#pragma unroll 4
-      for (long i = rl; i < rows; i += RED_R) tr += (double)r[i * C + c];
+    constexpr int U = 8;
+    for (long i = rl; i < rows; i += U * RED_R) {
+      float x[U], y[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long k = min(i + u * RED_R, rows - 1) * C + c;
+        x[u] = q[k];
+        y[u] = TWO ? r[k] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool on = i + u * RED_R < rows;
+        t[0] += on ? (double)x[u] : 0.0;
+        if (TWO) t[1] += on ? (double)y[u] : 0.0;
+      }
+    }
   }
-  vq = vr = 0.0;
-  red[rl][cl] = tq;
-  __syncthreads();
-  if (rl == 0)
-#pragma unroll 8
-    for (int i = 0; i < RED_R; ++i) vq += red[i][cl];
-  if (!r) return;                       // (the same for every thread)
-  __syncthreads();
-  red[rl][cl] = tr;
-  __syncthreads();
-  if (rl == 0)
-#pragma unroll 8
-    for (int i = 0; i < RED_R; ++i) vr += red[i][cl];
+  double v[2] = {0.0, 0.0};
+#pragma unroll
+  for (int k = 0; k < (TWO ? 2 : 1); ++k) {
+    __syncthreads();
+    red[rl][cl] = t[k];
+    __syncthreads();
+    if (rl == 0)
+#pragma unroll 16
+      for (int i = 0; i < RED_R; ++i) v[k] += red[i][cl];
+  }
+  vq = v[0];
+  vr = v[1];
 }
 __device__ __forceinline__ void reduce_out(float* out, long c, double v, int accumulate) {
   if (out) out[c] = accumulate ? (float)((double)out[c] + v) : (float)v;
@@ -218,30 +231,36 @@ __global__ __launch_bounds__(RED_C * RED_R) void rn_reduce(const ReduceArgs a) {
   double v0, v1;
   if (blockIdx.y == 0) {
     if (!a.dpost_w && !a.dpost_b && !a.dgate) return;
+    const float *g1 = a.part + RN_Q_G1 * plane, *g0 = a.part + RN_Q_G0 * plane;
     const bool g1_used = a.dpost_w || a.dgate, g0_used = a.dpost_b || (a.dgate && a.post_b);
-    reduce_columns(g1_used ? a.part + RN_Q_G1 * plane : nullptr, g0_used ? a.part + RN_Q_G0 * plane : nullptr, a.rows, a.C, c, red, v0, v1);
+    if (g1_used && g0_used) {
+      reduce_columns<true>(g1, g0, a.rows, a.C, c, red, v0, v1);
+    } else {
+      reduce_columns<false>(g1_used ? g1 : g0, nullptr, a.rows, a.C, c, red, v0, v1);
+      if (!g1_used) v1 = v0;
+    }
     if (!writer) return;
     const double g = a.gate ? (double)a.gate[c] : 1.0;
     reduce_out(a.dpost_w, c, g * v0, a.accumulate);
     reduce_out(a.dpost_b, c, g * v1, a.accumulate);
     reduce_out(a.dgate, c, a.has_post ? a.post_w[c] * v0 + (a.post_b ? a.post_b[c] * v1 : 0.0) : v0, a.accumulate);
-  } else {
+  } else if (blockIdx.y == 1) {
     if (!a.dpre_w && !a.dpre_b) return;
-    reduce_columns(a.dpre_w ? a.part + RN_Q_PRE_W * plane : nullptr, a.dpre_b ? a.part + RN_Q_PRE_B * plane : nullptr, a.rows, a.C, c, red,
-                   v0, v1);
+    const float *w = a.part + RN_Q_PRE_W * plane, *b = a.part + RN_Q_PRE_B * plane;
+    if (a.dpre_w && a.dpre_b) {
+      reduce_columns<true>(w, b, a.rows, a.C, c, red, v0, v1);
+    } else {
+      reduce_columns<false>(a.dpre_w ? w : b, nullptr, a.rows, a.C, c, red, v0, v1);
+      v1 = v0;
+    }
     if (!writer) return;
     reduce_out(a.dpre_w, c, v0, a.accumulate);
     reduce_out(a.dpre_b, c, v1, a.accumulate);
+  } else {
+    const long b = blockIdx.y - 2;
+    reduce_columns<false>(a.part_gate + b * a.S * a.C, nullptr, a.S, a.C, c, red, v0, v1);
+    if (writer) reduce_out(a.dgate_image + b * a.C, c, v0, a.accumulate);
   }
-}
-// dgate [B][C] from the [B][S][C] sums of a gate per image
-__global__ __launch_bounds__(RED_C * RED_R) void rn_reduce_gate(const float* __restrict__ part, long S, long C,
-                                                                float* __restrict__ dgate, int accumulate) {
-  __shared__ double red[RED_R][RED_C + 1];
-  const long c = (long)blockIdx.x * RED_C + threadIdx.x % RED_C;
-  double v, none;
-  reduce_columns(part + (long)blockIdx.y * S * C, nullptr, S, C, c, red, v, none);
-  if (threadIdx.x < RED_C && c < C) reduce_out(dgate + (long)blockIdx.y * C, c, v, accumulate);
 }
 
 }  // namespace
@@ -355,12 +374,12 @@ int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, lon
     RN_TYPE(dtype, rn_launch_bwd);
 #undef RN_ARGS
     if (params) {
+      const bool images = gate_kind == 2 && dgate && a.S > 1;
       const ReduceArgs r{a.part, a.part_rows, C, dpost_w, dpost_b, gate_kind == 1 ? dgate : nullptr, dpre_w, dpre_b,
-                         gate_kind == 1 ? gate : nullptr, post_w, post_kind == 1 ? post_b : nullptr, post_kind, accumulate};
-      hipLaunchKernelGGL(rn_reduce, dim3((unsigned)((C + RED_C - 1) / RED_C), 2), dim3(RED_C * RED_R), 0, s, r);
-      if (gate_kind == 2 && dgate && a.S > 1)
-        hipLaunchKernelGGL(rn_reduce_gate, dim3((unsigned)((C + RED_C - 1) / RED_C), (unsigned)B), dim3(RED_C * RED_R), 0, s, a.part_gate, (long)a.S,
-                           (long)C, dgate, accumulate);
+                         gate_kind == 1 ? gate : nullptr, post_w, post_kind == 1 ? post_b : nullptr, post_kind, accumulate,
+                         images ? a.part_gate : nullptr, images ? dgate : nullptr, a.S};
+      // (S > 1 only below a few thousand images)
+      hipLaunchKernelGGL(rn_reduce, dim3((unsigned)((C + RED_C - 1) / RED_C), images ? 2u + B : 2u), dim3(RED_C * RED_R), 0, s, r);
     }
     JIRF_HIP_CHECK(hipGetLastError());
     return JIRF_OK;
