@@ -24,15 +24,15 @@ struct RnArgs {
   int post, pre, gate_kind, accumulate;
   float eps;
   int B, C, P;
-  // Workers: S per image, each a run of `per` tiles (ipw == 1), or one per ipw images (S == 1).
-  int S, ipw, per, tiles;
+  // Workers: S per image, each with every S-th tile (ipw == 1), or one per ipw images (S == 1).
+  int S, ipw, tiles;
 };
 // The branch's parameter gradients come from two sums per channel, G1 = sum s dyt vh and G0 = sum s dyt (vh = the
 // normalised f, or f): dpost_w = gate G1, dpost_b = gate G0, dgate = post_w G1 + post_b G0 (or G1 without a norm).
 // With a gate per image the factors belong inside the sum over the images: then the sums are dpost_w and dpost_b.
 enum { RN_Q_G1 = 0, RN_Q_G0 = 1, RN_Q_PRE_W = 2, RN_Q_PRE_B = 3, RN_Q_N = 4 };
 
-// Which kernel serves a call.  lanes: tokens - threads per token (8..64, several tokens per wave) or 0 (the whole
+// Which kernel serves a call.  lanes: tokens - threads per token (4..64, several tokens per wave) or 0 (the whole
 // workgroup); planar - pixel lanes; -1: the sweep form.
 struct RnForm {
   bool tok;
@@ -91,11 +91,17 @@ __device__ __forceinline__ void store_vec(char* image, unsigned off, int own, co
   }
 }
 
+#ifndef RN_FW
+#define RN_FW
+#endif
+#ifndef RN_BW
+#define RN_BW
+#endif
 constexpr int RN_T = 512;         // most threads of a workgroup in the register form (256 registers each)
 constexpr int RN_LANE_T = 256;    // threads of a workgroup whose waves hold several tokens each
 
 // ---- a tile in registers ------------------------------------------------------------------------------------------------
-// A worker owns a run of tiles; every thread holds NV vectors of VEC elements of each operand of a tile, so an operand is
+// A worker owns a set of tiles; every thread holds NV vectors of VEC elements of each operand of a tile, so an operand is
 // read once.  tokens: a tile is one token, a vector VEC consecutive channels, and the token's threads are L lanes of a
 // wave (a worker per lane group) or the workgroup (L == 0).  planar: a tile is L * VEC pixels of all channels, a vector VEC
 // consecutive pixels of one channel; L lanes run along the pixels, the other threads along the channels.
@@ -245,39 +251,39 @@ struct Tile {
 #pragma unroll
     for (int s = 0; s < NS; ++s) rs[s] = 1.0f / sqrtf(fmaf(rs[s], inv, a.eps));
   }
-  // images [b0, b1) and tiles [t0, t1) of worker w
-  __device__ __forceinline__ void range(long w, int& b0, int& b1, int& t0, int& t1, int& slab) const {
+  // images [b0, b1) of worker w, and its first tile in each: it takes every a.S-th from there
+  __device__ __forceinline__ void range(long w, int& b0, int& b1, int& t0) const {
     if (a.S > 1) {
       b0 = (int)min(w / a.S, (long)a.B);
       b1 = min(b0 + 1, a.B);
-      slab = (int)(w % a.S);
-      t0 = min(a.tiles, slab * a.per);
-      t1 = min(a.tiles, t0 + a.per);
+      t0 = (int)(w % a.S);
     } else {
       b0 = (int)min(w * a.ipw, (long)a.B);
       b1 = (int)min(w * a.ipw + a.ipw, (long)a.B);
-      slab = 0;
       t0 = 0;
-      t1 = a.tiles;
     }
   }
+  // Workers are numbered along each XCD: neighbours, which share the cache lines at the tiles' edges (planar rows are rarely
+  // whole lines, and a tile's piece of a row may be half of one), run at the same time on the same L2.
   __device__ __forceinline__ long worker() const {
-    if (TOK && L) return (long)blockIdx.x * (blockDim.x / L) + threadIdx.x / L;
-    return blockIdx.x;
+    const long block = xcd_remap(blockIdx.x, gridDim.x);
+    if (TOK && L) return block * (blockDim.x / L) + threadIdx.x / L;
+    return block;
   }
 };
 
 // Forward.  Reads x and f once and writes y and n once; the next tile's loads are issued before this tile's reductions.
 // The branch's factors are folded: u = vh (gate w) + gate b.
 template <typename T, bool TOK, int L, int NV, int VEC>
-__global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
+__global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_FW) void rn_fwd_tile(const RnArgs a) {
   typedef Tile<T, TOK, L, NV, VEC> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
   __shared__ float lds[Ti::RED];
   Ti ti(a, lds);
-  int b0, b1, t0, t1, slab;
-  ti.range(ti.worker(), b0, b1, t0, t1, slab);
+  int b0, b1, t0;
+  ti.range(ti.worker(), b0, b1, t0);
+  const int t1 = a.tiles;
   if (b0 >= b1 || t0 >= t1) return;           // (uniform over the threads of a worker, and a worker's barriers are its own)
   float pw[NV][NP], pb[NV][NP], gw[NV][NP], gb[NV][NP];
   Vec xn[NV], fn[NV];
@@ -304,14 +310,14 @@ __global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
       }
     }
     const float s = a.scale ? a.scale[b] : 1.0f;
-    for (int t = t0; t < t1; ++t) {
+    for (int t = t0; t < t1; t += a.S) {
       Vec xv[NV], fv[NV];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         xv[j] = xn[j];
         fv[j] = fn[j];
       }
-      const int bn = t + 1 < t1 ? b : b + 1, tn = t + 1 < t1 ? t + 1 : t0;
+      const int bn = t + a.S < t1 ? b : b + 1, tn = t + a.S < t1 ? t + a.S : t0;
       if (bn < b1) {
         ti.load(Ti::image(a.f, a.f_bs, bn), ti.start(tn), fn);
         ti.load(Ti::image(a.x, a.x_bs, bn), ti.start(tn), xn);
@@ -366,7 +372,7 @@ __global__ __launch_bounds__(RN_T) void rn_fwd_tile(const RnArgs a) {
 // Backward.  Every operand once; the parameter gradients accumulate in the registers of the threads that hold the
 // channel, over all of the worker's tiles, and are added up across lanes and waves once, at the end.
 template <typename T, bool TOK, int L, int NV, int VEC, int MODE>
-__global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
+__global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_BW) void rn_bwd_tile(const RnArgs a) {
   typedef Tile<T, TOK, L, NV, VEC> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
@@ -377,8 +383,9 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
   __shared__ float lds[Ti::RED];
   __shared__ float wsum[TOK && L ? RN_LANE_T / 64 * L * EW : 1];
   Ti ti(a, lds);
-  int b0, b1, t0, t1, slab;
-  ti.range(ti.worker(), b0, b1, t0, t1, slab);
+  int b0, b1, t0;
+  ti.range(ti.worker(), b0, b1, t0);
+  const int slab = t0, t1 = a.tiles;
   if (t0 >= t1) b1 = b0;                                       // nothing to do, but its partial sums are written (zeros)
   float acc[RN_Q_N][NV][NP], img[2][NV][NP];                   // img: G1, G0 of the current image
 #pragma unroll
@@ -448,7 +455,7 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
         for (int i = 0; i < NP; ++i) gw[j][i] = ti.exists(j, i) ? gw[j][i] * g[j][i] : 0.f;
     }
     const float s = a.scale ? a.scale[b] : 1.0f;
-    for (int t = t0; t < t1; ++t) {
+    for (int t = t0; t < t1; t += a.S) {
       if (!PF) fetch(b, t);
       Vec dy[NV], dn[NV], yv[NV], fv[NV];
 #pragma unroll
@@ -466,7 +473,7 @@ __global__ __launch_bounds__(RN_T) void rn_bwd_tile(const RnArgs a) {
         mu1[i] = sn[2][i];
         rs1[i] = sn[3][i];
       }
-      const int bn = t + 1 < t1 ? b : b + 1, tn = t + 1 < t1 ? t + 1 : t0;
+      const int bn = t + a.S < t1 ? b : b + 1, tn = t + a.S < t1 ? t + a.S : t0;
       if (PF && bn < b1) fetch(bn, tn);
       const unsigned st = ti.start(t);
       const int px = ti.own_pixels(t);
@@ -826,7 +833,7 @@ __global__ __launch_bounds__(256) void rn_bwd_params_sweep(const RnArgs a) {
   const int worker = blockIdx.y;
   const int b0 = a.S > 1 ? worker / a.S : worker * a.ipw, b1 = min(a.B, a.S > 1 ? b0 + 1 : b0 + a.ipw);
   const int slab = a.S > 1 ? worker % a.S : 0;
-  const long p0 = min((long)a.P, (long)slab * a.per * 64), p1 = a.S > 1 ? min((long)a.P, p0 + (long)a.per * 64) : a.P;
+  const long per = ((long)a.P + a.S - 1) / a.S, p0 = min((long)a.P, slab * per), p1 = min((long)a.P, p0 + per);
   const long bp = (long)a.B * a.P;
   const int c = blockIdx.x * (TOK ? 64 : 4) + (TOK ? lane : wave);
   const bool on = c < a.C;
@@ -913,6 +920,7 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
     else hipLaunchKernelGGL((rn_fwd_sweep<T, false>), dim3(sweep_blocks(false, a.B, a.P)), dim3(256), 0, s, a);
   } else if (f.tok) {
     switch (f.lanes) {
+      case 4: RN_FWD(true, 4, E8); break;
       case 8: RN_FWD(true, 8, E8); break;
       case 16: RN_FWD(true, 16, E8); break;
       case 32: RN_FWD(true, 32, E8); break;
@@ -940,6 +948,7 @@ void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
   constexpr int E8 = 8 / rn_vec<T>(true);
   if (f.tok) {
     switch (f.lanes) {
+      case 4: RN_BWD(true, 4, E8); break;
       case 8: RN_BWD(true, 8, E8); break;
       case 16: RN_BWD(true, 16, E8); break;
       case 32: RN_BWD(true, 32, E8); break;

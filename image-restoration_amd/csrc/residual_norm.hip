@@ -115,7 +115,7 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
     const int threads8 = (a.C + 7) / 8;
     f.nv = 8 / vec;
     if (threads8 <= 64) {
-      f.lanes = threads8 <= 8 ? 8 : threads8 <= 16 ? 16 : threads8 <= 32 ? 32 : 64;
+      f.lanes = threads8 <= 4 ? 4 : threads8 <= 8 ? 8 : threads8 <= 16 ? 16 : threads8 <= 32 ? 32 : 64;
       f.threads = 256;
       per_block = f.threads / f.lanes;
     } else if (threads8 <= 512) {
@@ -146,11 +146,10 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
   const long want = (f.lanes < 0 ? 256 : (backward ? 512 : 2048) * 256 / f.threads) * per_block;
   if (a.B >= want) {
     a.ipw = (int)((a.B + want - 1) / want);
-    a.per = a.tiles;
   } else {
-    const long S = std::max<long>(1, std::min<long>(a.tiles, want / a.B));
-    a.per = (int)((a.tiles + S - 1) / S);
-    a.S = (int)((a.tiles + a.per - 1) / a.per);
+    // the same number of tiles for every worker, but the last few
+    const long S = std::max<long>(1, std::min<long>(a.tiles, want / a.B)), rounds = (a.tiles + S - 1) / S;
+    a.S = (int)((a.tiles + rounds - 1) / rounds);
   }
   const long workers = a.S > 1 ? (long)a.B * a.S : ((long)a.B + a.ipw - 1) / a.ipw;
   f.blocks = (unsigned)((workers + per_block - 1) / per_block);
