@@ -73,32 +73,71 @@ template <typename T, int VEC> struct Pack {
   __device__ __forceinline__ void load(const char* image, unsigned off) { v = *reinterpret_cast<const VU*>(image + off); }
   __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
 };
-// the last `own` of VEC values
 template <typename T, int VEC>
-__device__ __forceinline__ void store_vec(char* image, unsigned off, int own, const float* f) {
+__device__ __forceinline__ void store_vec(char* image, unsigned off, const float* f) {
   typedef T V __attribute__((ext_vector_type(VEC)));
   typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   V v;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) v[i] = (T)f[i];
-  T* p = reinterpret_cast<T*>(image + off);
+  *reinterpret_cast<VU*>(image + off) = v;
+}
+// the last `own` of VEC values
+template <typename T, int VEC>
+__device__ __forceinline__ void store_some(char* image, unsigned off, int own, const float* f) {
   if (own == VEC) {
-    *reinterpret_cast<VU*>(p) = v;
+    store_vec<T, VEC>(image, off, f);
   } else {
+    T* p = reinterpret_cast<T*>(image + off);
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
-      if (i >= VEC - own) p[i] = v[i];
+      if (i >= VEC - own) p[i] = (T)f[i];
   }
 }
 
-#ifndef RN_FW
-#define RN_FW
-#endif
-#ifndef RN_BW
-#define RN_BW
-#endif
 constexpr int RN_T = 512;         // most threads of a workgroup in the register form (256 registers each)
 constexpr int RN_LANE_T = 256;    // threads of a workgroup whose waves hold several tokens each
+
+// x + the value of another lane, by one data-parallel instruction (no LDS access, as a shuffle makes).
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float add_row16(float x) {       // rows of 16 lanes, in pairs
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_half32(float x) {      // the two halves of the wave
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The sum over the lanes i, i + STRIDE, i + 2 STRIDE, ... of a group of SIZE lanes, in every one of them.
+template <int STRIDE, int SIZE>
+__device__ __forceinline__ float lane_sum(float x) {
+  if constexpr (SIZE == 4 || SIZE == 8) {
+    static_assert(STRIDE == 1, "");
+    x = add_dpp<0xB1>(x);                                   // lane ^ 1
+    x = add_dpp<0x4E>(x);                                   // lane ^ 2
+    if constexpr (SIZE == 8) x = add_dpp<0x141>(x);         // lane 7 - i of the eight: the other four's sum
+  } else {
+    if constexpr (STRIDE <= 8) x = add_dpp<0x128>(x);       // rotations inside the row of 16
+    if constexpr (STRIDE <= 4) x = add_dpp<0x124>(x);
+    if constexpr (STRIDE <= 2) x = add_dpp<0x122>(x);
+    if constexpr (STRIDE <= 1) x = add_dpp<0x121>(x);
+    if constexpr (SIZE >= 32 && STRIDE <= 16) x = add_row16(x);
+    if constexpr (SIZE >= 64) x = add_half32(x);
+  }
+  return x;
+}
+// 1 / sqrt(x), correctly rounded: the hardware's estimate and one Newton step whose residual 1 - x y^2 is formed without
+// rounding error (product and its remainder apart); small x scaled into the estimate's range, 0 and infinity as they are.
+__device__ __forceinline__ float recip_sqrt(float x) {
+  const bool tiny = x < 0x1p-96f;
+  x *= tiny ? 0x1p64f : 1.0f;
+  const float y = __builtin_amdgcn_rsqf(x), p = x * y, lo = fmaf(x, y, -p);
+  const float e = fmaf(-lo, y, fmaf(-p, y, 1.0f)), r = fmaf(0.5f * y, e, y);
+  return (y > 0.f && y < __builtin_inff() ? r : y) * (tiny ? 0x1p32f : 1.0f);
+}
 
 // ---- a tile in registers ------------------------------------------------------------------------------------------------
 // A worker owns a set of tiles; every thread holds NV vectors of VEC elements of each operand of a tile, so an operand is
@@ -127,7 +166,7 @@ struct Tile {
     const int tid = threadIdx.x;
     if (TOK) {
       ch = L ? tid & (L - 1) : tid;
-      nch = L ? L : blockDim.x;
+      nch = L ? L : (int)blockDim.x;
       pl = 0;
     } else {
       pl = tid & (L - 1);
@@ -168,12 +207,19 @@ struct Tile {
 #pragma unroll
     for (int j = 0; j < NV; ++j) r[j].load(img, st + off[j]);
   }
-  __device__ __forceinline__ void store(void* p, long bs, int b, unsigned st, int px, const float (&f)[NV][VEC]) const {
+  // whether some vector of tile t is shared (the same answer for the whole workgroup)
+  __device__ __forceinline__ bool edge(int t) const { return TOK ? a.C % VEC != 0 : (long)(t + 1) * (L * VEC) > a.P; }
+  __device__ __forceinline__ void store(void* p, long bs, int b, int t, const float (&f)[NV][VEC]) const {
     char* img = const_cast<char*>(image(p, bs, b));
+    const unsigned st = start(t);
+    if (!edge(t)) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int n = TOK ? own[j] : own[j] ? px : 0;
-      if (n > 0) store_vec<T, VEC>(img, st + off[j], n, f[j]);
+      for (int j = 0; j < NV; ++j)
+        if (own[j]) store_vec<T, VEC>(img, st + off[j], f[j]);
+    } else {
+      const int px = own_pixels(t);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) store_some<T, VEC>(img, st + off[j], TOK ? own[j] : own[j] ? px : 0, f[j]);
     }
   }
   // a [C] array in the thread's channels; `none` for a channel that is not its own, or without an array
@@ -197,32 +243,25 @@ struct Tile {
   // one barrier per reduction is enough.
   template <int N>
   __device__ __forceinline__ void reduce(float (&v)[N]) {
-    if (TOK && L) {
+    constexpr int W = TOK ? 1 : L;
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
-      return;
-    }
-#pragma unroll
-    for (int o = 32; o >= (TOK ? 1 : L); o >>= 1)
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    for (int i = 0; i < N; ++i) v[i] = lane_sum<W, TOK && L ? L : 64>(v[i]);
+    if (TOK && L) return;
     const int waves = blockDim.x >> 6, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     if (waves == 1) return;
-    constexpr int W = TOK ? 1 : L;
-    float* r = red + buf * (RED / 2);
+    typedef float F __attribute__((ext_vector_type(N)));
+    F* r = reinterpret_cast<F*>(red + buf * (RED / 2));
     buf ^= 1;
-    if (lane < W)
+    F q;
 #pragma unroll
-      for (int i = 0; i < N; ++i) r[(wave * W + lane) * N + i] = v[i];
+    for (int i = 0; i < N; ++i) q[i] = v[i];
+    if (lane < W) r[wave * W + lane] = q;
     __syncthreads();
     const int at = TOK ? 0 : pl;
+    q = r[at];
+    for (int w = 1; w < waves; ++w) q += r[w * W + at];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = r[at * N + i];
-    for (int w = 1; w < waves; ++w)
-#pragma unroll
-      for (int i = 0; i < N; ++i) v[i] += r[(w * W + at) * N + i];
+    for (int i = 0; i < N; ++i) v[i] = q[i];
   }
   // mean (0 for the root mean square) and reciprocal deviation, in two passes over the registers
   __device__ __forceinline__ void statistics(const float (&v)[NV][VEC], int kind, float (&mu)[NS], float (&rs)[NS]) {
@@ -232,8 +271,9 @@ struct Tile {
     if (kind != 3) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
+        if (TOK || own[j])
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) mu[TOK ? 0 : i] += exists(j, i) ? v[j][i] : 0.f;
+          for (int i = 0; i < VEC; ++i) mu[TOK ? 0 : i] += !TOK || exists(j, i) ? v[j][i] : 0.f;
       reduce<NS>(mu);
 #pragma unroll
       for (int s = 0; s < NS; ++s) mu[s] *= inv;
@@ -242,14 +282,15 @@ struct Tile {
     for (int s = 0; s < NS; ++s) rs[s] = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
+      if (TOK || own[j])
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = exists(j, i) ? v[j][i] - mu[TOK ? 0 : i] : 0.f;
-        rs[TOK ? 0 : i] = fmaf(d, d, rs[TOK ? 0 : i]);
-      }
+        for (int i = 0; i < VEC; ++i) {
+          const float d = !TOK || exists(j, i) ? v[j][i] - mu[TOK ? 0 : i] : 0.f;
+          rs[TOK ? 0 : i] = fmaf(d, d, rs[TOK ? 0 : i]);
+        }
     reduce<NS>(rs);
 #pragma unroll
-    for (int s = 0; s < NS; ++s) rs[s] = 1.0f / sqrtf(fmaf(rs[s], inv, a.eps));
+    for (int s = 0; s < NS; ++s) rs[s] = recip_sqrt(fmaf(rs[s], inv, a.eps));
   }
   // images [b0, b1) of worker w, and its first tile in each: it takes every a.S-th from there
   __device__ __forceinline__ void range(long w, int& b0, int& b1, int& t0) const {
@@ -267,7 +308,7 @@ struct Tile {
   // whole lines, and a tile's piece of a row may be half of one), run at the same time on the same L2.
   __device__ __forceinline__ long worker() const {
     const long block = xcd_remap(blockIdx.x, gridDim.x);
-    if (TOK && L) return block * (blockDim.x / L) + threadIdx.x / L;
+    if (TOK && L) return block * (RN_LANE_T / (L ? L : 1)) + threadIdx.x / (L ? L : 1);
     return block;
   }
 };
@@ -275,11 +316,11 @@ struct Tile {
 // Forward.  Reads x and f once and writes y and n once; the next tile's loads are issued before this tile's reductions.
 // The branch's factors are folded: u = vh (gate w) + gate b.
 template <typename T, bool TOK, int L, int NV, int VEC>
-__global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_FW) void rn_fwd_tile(const RnArgs a) {
+__global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_fwd_tile(const RnArgs a) {
   typedef Tile<T, TOK, L, NV, VEC> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
-  __shared__ float lds[Ti::RED];
+  __shared__ __attribute__((aligned(16))) float lds[Ti::RED];
   Ti ti(a, lds);
   int b0, b1, t0;
   ti.range(ti.worker(), b0, b1, t0);
@@ -322,7 +363,6 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_FW) void rn_fwd_tile
         ti.load(Ti::image(a.f, a.f_bs, bn), ti.start(tn), fn);
         ti.load(Ti::image(a.x, a.x_bs, bn), ti.start(tn), xn);
       }
-      const unsigned st = ti.start(t);
       const int px = ti.own_pixels(t);
       float v[NV][VEC], mu0[NS], rs0[NS], mu1[NS], rs1[NS];
 #pragma unroll
@@ -343,7 +383,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_FW) void rn_fwd_tile
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
           v[j][i] = fmaf(s, fmaf(v[j][i], gw[j][TOK ? i : 0], gb[j][TOK ? i : 0]), xv[j].at(i));
-      ti.store(a.y, a.y_bs, b, st, px, v);
+      ti.store(a.y, a.y_bs, b, t, v);
       if (a.pre) {
         ti.statistics(v, a.pre, mu1, rs1);
 #pragma unroll
@@ -351,7 +391,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_FW) void rn_fwd_tile
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
             v[j][i] = fmaf((a.pre == 1 ? v[j][i] - mu1[TOK ? 0 : i] : v[j][i]) * rs1[TOK ? 0 : i], pw[j][TOK ? i : 0], pb[j][TOK ? i : 0]);
-        ti.store(a.n, a.n_bs, b, st, px, v);
+        ti.store(a.n, a.n_bs, b, t, v);
       }
       if (a.stats && ti.ch == 0) {
         const long bp = (long)a.B * a.P;
@@ -372,7 +412,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_FW) void rn_fwd_tile
 // Backward.  Every operand once; the parameter gradients accumulate in the registers of the threads that hold the
 // channel, over all of the worker's tiles, and are added up across lanes and waves once, at the end.
 template <typename T, bool TOK, int L, int NV, int VEC, int MODE>
-__global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_BW) void rn_bwd_tile(const RnArgs a) {
+__global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_bwd_tile(const RnArgs a) {
   typedef Tile<T, TOK, L, NV, VEC> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
@@ -380,7 +420,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_BW) void rn_bwd_tile
   constexpr int EW = NV * NP;                                  // channels of a thread
   // the next tile's operands are fetched ahead where the registers (256 per thread) have room for two tiles
   constexpr bool PF = !(BR && NV * VEC == 16 && (sizeof(T) == 4 || IG));
-  __shared__ float lds[Ti::RED];
+  __shared__ __attribute__((aligned(16))) float lds[Ti::RED];
   __shared__ float wsum[TOK && L ? RN_LANE_T / 64 * L * EW : 1];
   Ti ti(a, lds);
   int b0, b1, t0;
@@ -475,7 +515,6 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_BW) void rn_bwd_tile
       }
       const int bn = t + a.S < t1 ? b : b + 1, tn = t + a.S < t1 ? t + a.S : t0;
       if (PF && bn < b1) fetch(bn, tn);
-      const unsigned st = ti.start(t);
       const int px = ti.own_pixels(t);
       // a pixel that is not the vector's own is all zeros below, whatever stands there: it adds nothing to any sum
 #pragma unroll
@@ -519,7 +558,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_BW) void rn_bwd_tile
 #pragma unroll
           for (int i = 0; i < VEC; ++i) d[j][i] = dy[j].at(i);
       }
-      ti.store(a.dx, a.dx_bs, b, st, px, d);
+      ti.store(a.dx, a.dx_bs, b, t, d);
       if (!BR) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -559,7 +598,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T RN_BW) void rn_bwd_tile
             }
         }
       }
-      ti.store(a.df, a.df_bs, b, st, px, d);
+      ti.store(a.df, a.df_bs, b, t, d);
     }
     if (IG) {
       // the image is done: its gate's gradient, and its share of the norm's parameters

@@ -113,12 +113,13 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
   } else if (f.tok) {
     // eight channels per thread; sixteen where eight would need more than 512 threads
     const int threads8 = (a.C + 7) / 8;
+    const bool wide16 = backward && dtype != JIRF_F32 && a.gate_kind != 2 && (a.post || a.gate_kind);
     f.nv = 8 / vec;
     if (threads8 <= 64) {
       f.lanes = threads8 <= 4 ? 4 : threads8 <= 8 ? 8 : threads8 <= 16 ? 16 : threads8 <= 32 ? 32 : 64;
       f.threads = 256;
       per_block = f.threads / f.lanes;
-    } else if (threads8 <= 512) {
+    } else if (threads8 <= (wide16 ? 256 : 512)) {
       f.threads = (threads8 + 63) / 64 * 64;
     } else if (a.C <= 8192) {
       f.nv *= 2;
@@ -143,7 +144,12 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
   // Workers: enough workgroups to fill the chip several times over (forward), or about twice (backward: each leaves a row
   // of partial sums per parameter).
   if (f.lanes < 0) a.tiles = (int)(((long)a.P + 63) / 64);
-  const long want = (f.lanes < 0 ? 256 : (backward ? 512 : 2048) * 256 / f.threads) * per_block;
+  long want = 256;
+  if (f.lanes >= 0) {
+    if (backward) want = 256 * std::max(1, 512 / f.threads);
+    else want = f.threads < 256 ? 2048 * 256 / f.threads : f.lanes == 0 ? 256 * (1024 / f.threads) : 2048;
+  }
+  want *= per_block;
   if (a.B >= want) {
     a.ipw = (int)((a.B + want - 1) / want);
   } else {
