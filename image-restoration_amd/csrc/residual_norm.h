@@ -96,6 +96,7 @@ __device__ __forceinline__ void store_some(char* image, unsigned off, int own, c
 }
 
 constexpr int RN_T = 512;         // most threads of a workgroup in the register form (256 registers each)
+constexpr int RN_T16 = 1024;      // the same for the planar forward of 16-bit types (128 registers each)
 constexpr int RN_LANE_T = 256;    // threads of a workgroup whose waves hold several tokens each
 
 // x + the value of another lane, by one data-parallel instruction (no LDS access, as a shuffle makes).
@@ -160,7 +161,8 @@ struct Tile {
   int own[NV];                                   // tokens: elements of each vector that are its own; planar: 1 or 0
   unsigned off[NV];                              // bytes from the token's first channel / from the image's first pixel 0
 
-  static constexpr int RED = TOK ? (L ? 1 : 2 * 8 * 2) : 2 * 8 * L * 2 * VEC;
+  // two buffers of [waves][token lanes][two sums per statistic]
+  static constexpr int RED = TOK ? (L ? 1 : 2 * (RN_T / 64) * 2) : 2 * (RN_T16 / 64) * L * 2 * VEC;
 
   __device__ __forceinline__ Tile(const RnArgs& args, float* lds) : a(args), red(lds), buf(0) {
     const int tid = threadIdx.x;
@@ -316,7 +318,7 @@ struct Tile {
 // Forward.  Reads x and f once and writes y and n once; the next tile's loads are issued before this tile's reductions.
 // The branch's factors are folded: u = vh (gate w) + gate b.
 template <typename T, bool TOK, int L, int NV, int VEC>
-__global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_fwd_tile(const RnArgs a) {
+__global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_T16 : RN_T) void rn_fwd_tile(const RnArgs a) {
   typedef Tile<T, TOK, L, NV, VEC> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;

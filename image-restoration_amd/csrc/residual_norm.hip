@@ -129,25 +129,28 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
     }
   } else {
     // four channels of four pixels per thread: as many pixel lanes (of 32) as the channels leave room for in 256 threads,
-    // more threads only to keep eight lanes (a 128-byte line of fp32) or, past that, any
-    const int rows = (a.C + 3) / 4;
+    // more threads only to keep eight lanes (a 128-byte line of fp32), or fewer lanes than that to fit at all
+    const int rows = (a.C + 3) / 4, most = !backward && dtype != JIRF_F32 ? 1024 : 512;
     f.nv = 4;
     f.lanes = 32;
     while (f.lanes > 8 && f.lanes * rows > 256) f.lanes >>= 1;
-    while (f.lanes > 2 && f.lanes * rows > 512) f.lanes >>= 1;
+    while (f.lanes > 2 && f.lanes * rows > most) f.lanes >>= 1;
     // no wider than the plane, and narrower while the tiles leave CUs idle
     while (f.lanes > 4 && (f.lanes * 2 >= a.P || ((long)a.P + f.lanes * 4 - 1) / (f.lanes * 4) * a.B < 256)) f.lanes >>= 1;
     f.threads = std::max(64, (f.lanes * rows + 63) / 64 * 64);
-    if (f.threads > 512) f.lanes = -1;
+    if (f.threads > most) f.lanes = -1;
     else a.tiles = (int)(((long)a.P + f.lanes * 4 - 1) / (f.lanes * 4));
   }
-  // Workers: enough workgroups to fill the chip several times over (forward), or about twice (backward: each leaves a row
-  // of partial sums per parameter).
+  // Workers.  Workgroups of a kernel that loops over its tiles are best all resident at once (256 CUs, and a CU holds 8 waves
+  // of the backward's 256 registers, 16 and more of the forward's); more and smaller ones only while they are small.  Tokens
+  // 4x4096x2048 bf16 backward (256 threads): 256 / 512 / 1024 workgroups 143 / 94 / 108 us; 4x1066x3344 fp16: 512 threads
+  // 37 / 41 / 51 us; planar 13x153x21471 fp16 forward (320 threads): 512 / 1024 / 2048 114 / 141 / 132 us.  In the
+  // backward each also leaves a row of partial sums.
   if (f.lanes < 0) a.tiles = (int)(((long)a.P + 63) / 64);
   long want = 256;
   if (f.lanes >= 0) {
     if (backward) want = 256 * std::max(1, 512 / f.threads);
-    else want = f.threads < 256 ? 2048 * 256 / f.threads : f.lanes == 0 ? 256 * (1024 / f.threads) : 2048;
+    else want = f.threads <= 256 ? 2048 : f.threads <= 512 ? 512 : 256;
   }
   want *= per_block;
   if (a.B >= want) {
