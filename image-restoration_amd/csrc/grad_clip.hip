@@ -92,8 +92,13 @@ __device__ __forceinline__ f32x8 clip_widen(const Raw<TY>& r) {
   }
   return v;
 }
-// rounded to nearest even
-template <int TY>
+// rounded to nearest even; NT: not kept in the caches
+template <typename V, bool NT, typename U>
+__device__ __forceinline__ void clip_put(void* p, unsigned byte, U v) {
+  if (NT) __builtin_nontemporal_store((V)v, dev<V>(p, byte));
+  else *dev<V>(p, byte) = v;
+}
+template <int TY, bool NT = false>
 __device__ __forceinline__ void clip_store8(void* p, unsigned g, const f32x8& v) {
   if constexpr (TY == TY_F32) {
     u32x4 a, b;
@@ -102,18 +107,18 @@ __device__ __forceinline__ void clip_store8(void* p, unsigned g, const f32x8& v)
       a[i] = __float_as_uint(v[i]);
       b[i] = __float_as_uint(v[4 + i]);
     }
-    *dev<u32x4_a4>(p, g * 32u) = a;
-    *dev<u32x4_a4>(p, g * 32u + 16u) = b;
+    clip_put<u32x4_a4, NT>(p, g * 32u, a);
+    clip_put<u32x4_a4, NT>(p, g * 32u + 16u, b);
   } else if constexpr (TY == TY_BF16) {
     bf16x8 h;
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = (__bf16)v[i];
-    *dev<u32x4_a2>(p, g * 16u) = __builtin_bit_cast(u32x4, h);
+    clip_put<u32x4_a2, NT>(p, g * 16u, __builtin_bit_cast(u32x4, h));
   } else {
     f16x8 h;
 #pragma unroll
     for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i];
-    *dev<u32x4_a2>(p, g * 16u) = __builtin_bit_cast(u32x4, h);
+    clip_put<u32x4_a2, NT>(p, g * 16u, __builtin_bit_cast(u32x4, h));
   }
 }
 template <int TY>
@@ -172,7 +177,7 @@ __device__ __forceinline__ void norm_any(const ClipChunk& ck, unsigned t, ClipAc
   else norm_chunk<MAX, TY_F16>(ck, t, acc);
 }
 
-template <int TS, int TD>
+template <bool NT, int TS, int TD>
 __device__ __forceinline__ void scale_chunk(const ClipChunk& ck, unsigned t, float k) {
   const unsigned groups = ck.n / CLIP_E;
   unsigned g = t;
@@ -181,26 +186,27 @@ __device__ __forceinline__ void scale_chunk(const ClipChunk& ck, unsigned t, flo
 #pragma unroll
     for (int u = 0; u < CLIP_U; ++u) r[u] = clip_load8<TS>(ck.src, g + u * CLIP_T);
 #pragma unroll
-    for (int u = 0; u < CLIP_U; ++u) clip_store8<TD>(ck.dst, g + u * CLIP_T, clip_widen<TS>(r[u]) * k);
+    for (int u = 0; u < CLIP_U; ++u) clip_store8<TD, NT>(ck.dst, g + u * CLIP_T, clip_widen<TS>(r[u]) * k);
   }
-  for (; g < groups; g += CLIP_T) clip_store8<TD>(ck.dst, g, clip_widen<TS>(clip_load8<TS>(ck.src, g)) * k);
+  for (; g < groups; g += CLIP_T) clip_store8<TD, NT>(ck.dst, g, clip_widen<TS>(clip_load8<TS>(ck.src, g)) * k);
   const unsigned i = groups * CLIP_E + t;
   if (i < ck.n) clip_store1<TD>(ck.dst, i, clip_load1<TS>(ck.src, i) * k);
 }
-template <int TS>
+template <bool NT, int TS>
 __device__ __forceinline__ void scale_to(const ClipChunk& ck, unsigned t, float k) {
   const unsigned td = ck.types >> 8;
-  if (td == TY_F32) scale_chunk<TS, TY_F32>(ck, t, k);
-  else if (td == TY_BF16) scale_chunk<TS, TY_BF16>(ck, t, k);
-  else scale_chunk<TS, TY_F16>(ck, t, k);
+  if (td == TY_F32) scale_chunk<NT, TS, TY_F32>(ck, t, k);
+  else if (td == TY_BF16) scale_chunk<NT, TS, TY_BF16>(ck, t, k);
+  else scale_chunk<NT, TS, TY_F16>(ck, t, k);
 }
+template <bool NT>
 __device__ __forceinline__ void scale_any(const ClipChunk& ck, unsigned t, float k) {
   const unsigned ts = ck.types & 0xff;
   // in place with factor 1 every value stays as it is
   if (k == 1.0f && ck.src == ck.dst && ts == ck.types >> 8) return;
-  if (ts == TY_F32) scale_to<TY_F32>(ck, t, k);
-  else if (ts == TY_BF16) scale_to<TY_BF16>(ck, t, k);
-  else scale_to<TY_F16>(ck, t, k);
+  if (ts == TY_F32) scale_to<NT, TY_F32>(ck, t, k);
+  else if (ts == TY_BF16) scale_to<NT, TY_BF16>(ck, t, k);
+  else scale_to<NT, TY_F16>(ck, t, k);
 }
 
 // Combines over the workgroup (butterfly in each wave, then the waves in order); the result in every thread.
@@ -253,7 +259,7 @@ __global__ __launch_bounds__(CLIP_T) void norm_kernel(const ClipChunk* __restric
 }
 
 // The chunks are taken from the last to the first: what norm_kernel read last is what the cache still holds.
-template <bool MAX>
+template <bool MAX, bool NT>
 __global__ __launch_bounds__(CLIP_T) void clip_kernel(const ClipChunk* __restrict__ chunks, int n_chunks,
                                                       const double* __restrict__ part, int n_part, double max_norm,
                                                       double grad_scale, double* __restrict__ stats) {
@@ -262,7 +268,7 @@ __global__ __launch_bounds__(CLIP_T) void clip_kernel(const ClipChunk* __restric
   for (int i = threadIdx.x; i < n_part; i += CLIP_T) t = combine2<MAX>(t, part[i]);
   const double raw = block_combine<MAX, CLIP_T>(t, red);
   const float k = clip_factor<MAX>(raw, max_norm, grad_scale, stats, blockIdx.x == 0 && threadIdx.x == 0);
-  for (int c = n_chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) scale_any(chunks[c], threadIdx.x, k);
+  for (int c = n_chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) scale_any<NT>(chunks[c], threadIdx.x, k);
 }
 
 // Small lists (at most CLIP_SMALL_E elements in CLIP_SMALL_CHUNKS chunks of CLIP_SMALL_T): one workgroup, one launch.  Teams
@@ -501,8 +507,13 @@ int jirf_train_grad_clip_run(const void* plan, int norm_kind, double max_norm, d
     }
     {
       Scope sc("train_grad_clip", 1.0 * pl->total, pl->writes ? pl->bytes_read + pl->bytes_written : 0.0, s);
-      hipLaunchKernelGGL(mx ? clip_kernel<true> : clip_kernel<false>, dim3(pl->writes ? pl->blocks : 1), dim3(CLIP_T), 0, s, ck,
-                         pl->writes ? pl->n_chunks : 0, work, pl->blocks, max_norm, grad_scale, stats);
+      // Past half of the 256 MB cache the stores go around it, to leave it to the gradients read a second time: 26.3 M
+      // fp32 values 67.9 -> 64.5 us, 536 M bf16 661 -> 645 us.
+      const bool nt = pl->bytes_read + pl->bytes_written > (128 << 20);
+      const auto kernel = mx ? (nt ? clip_kernel<true, true> : clip_kernel<true, false>)
+                             : (nt ? clip_kernel<false, true> : clip_kernel<false, false>);
+      hipLaunchKernelGGL(kernel, dim3(pl->writes ? pl->blocks : 1), dim3(CLIP_T), 0, s, ck, pl->writes ? pl->n_chunks : 0, work,
+                         pl->blocks, max_norm, grad_scale, stats);
     }
     JIRF_HIP_CHECK(hipGetLastError());
     return JIRF_OK;

@@ -35,7 +35,7 @@ enum { RN_Q_G1 = 0, RN_Q_G0 = 1, RN_Q_PRE_W = 2, RN_Q_PRE_B = 3, RN_Q_N = 4 };
 // Which kernel serves a call.  lanes: tokens - threads per token (4..64, several tokens per wave) or 0 (the whole
 // workgroup); planar - pixel lanes; -1: the sweep form.
 struct RnForm {
-  bool tok;
+  bool tok, stream;        // stream: operands larger than the caches, read past them
   int lanes, nv, threads;
   unsigned blocks;
 };
@@ -66,11 +66,15 @@ template <> struct Elem<_Float16> {
 
 // VEC consecutive elements, read and written at the alignment of one element (rows of odd length, channel slices: the
 // memory instructions take any 2- or 4-byte address), `off` bytes into an image.
-template <typename T, int VEC> struct Pack {
+// NT: read once and not kept in the caches.
+template <typename T, int VEC, bool NT> struct Pack {
   typedef T V __attribute__((ext_vector_type(VEC)));
   typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   V v;
-  __device__ __forceinline__ void load(const char* image, unsigned off) { v = *reinterpret_cast<const VU*>(image + off); }
+  __device__ __forceinline__ void load(const char* image, unsigned off) {
+    const VU* p = reinterpret_cast<const VU*>(image + off);
+    v = NT ? __builtin_nontemporal_load(p) : *p;
+  }
   __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
 };
 template <typename T, int VEC>
@@ -149,11 +153,11 @@ __device__ __forceinline__ float recip_sqrt(float x) {
 // none branches; the elements it then shares with its neighbour belong to the neighbour: they are left out of sums and
 // stores.  A thread without a channel repeats the last one and owns nothing.  Needs C >= VEC (tokens) or P >= VEC (planar),
 // and less than 2^32 bytes in an image.
-template <typename T, bool TOK, int L, int NV, int VEC>
+template <typename T, bool TOK, int L, int NV, int VEC, bool NT>
 struct Tile {
   static constexpr int NS = TOK ? 1 : VEC;       // statistics per thread: its token's, or one per pixel of its vector
   static constexpr int NP = TOK ? VEC : 1;       // parameters per vector
-  typedef Pack<T, VEC> Vec;
+  typedef Pack<T, VEC, NT> Vec;
   const RnArgs& a;
   float* red;                                    // LDS of two reductions
   int buf;
@@ -317,9 +321,9 @@ struct Tile {
 
 // Forward.  Reads x and f once and writes y and n once; the next tile's loads are issued before this tile's reductions.
 // The branch's factors are folded: u = vh (gate w) + gate b.
-template <typename T, bool TOK, int L, int NV, int VEC>
+template <typename T, bool TOK, int L, int NV, int VEC, bool NT>
 __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_T16 : RN_T) void rn_fwd_tile(const RnArgs a) {
-  typedef Tile<T, TOK, L, NV, VEC> Ti;
+  typedef Tile<T, TOK, L, NV, VEC, NT> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
   __shared__ __attribute__((aligned(16))) float lds[Ti::RED];
@@ -413,9 +417,9 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
 
 // Backward.  Every operand once; the parameter gradients accumulate in the registers of the threads that hold the
 // channel, over all of the worker's tiles, and are added up across lanes and waves once, at the end.
-template <typename T, bool TOK, int L, int NV, int VEC, int MODE>
+template <typename T, bool TOK, int L, int NV, int VEC, bool NT, int MODE>
 __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_bwd_tile(const RnArgs a) {
-  typedef Tile<T, TOK, L, NV, VEC> Ti;
+  typedef Tile<T, TOK, L, NV, VEC, NT> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
   constexpr bool BR = MODE != RN_BWD_STREAM, IG = MODE == RN_BWD_IMAGE_GATE;
@@ -951,8 +955,9 @@ unsigned sweep_blocks(bool tok, int B, int P) {
   return (unsigned)std::min<long>(tiles, 1 << 16);
 }
 
-#define RN_FWD(TOK, L, NV)                                                                                                \
-  hipLaunchKernelGGL((rn_fwd_tile<T, TOK, L, NV, rn_vec<T>(TOK)>), dim3(f.blocks), dim3(f.threads), 0, s, a)
+#define RN_FWD_NT(TOK, L, NV, NT)                                                                                         \
+  hipLaunchKernelGGL((rn_fwd_tile<T, TOK, L, NV, rn_vec<T>(TOK), NT>), dim3(f.blocks), dim3(f.threads), 0, s, a)
+#define RN_FWD(TOK, L, NV) RN_FWD_NT(TOK, L, NV, false)
 template <typename T>
 void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
   constexpr int E8 = 8 / rn_vec<T>(true);       // vectors for eight channels per thread
@@ -967,7 +972,9 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
       case 32: RN_FWD(true, 32, E8); break;
       case 64: RN_FWD(true, 64, E8); break;
       default:
-        if (f.nv == E8) RN_FWD(true, 0, E8);
+        if (f.nv == E8 && f.stream) RN_FWD_NT(true, 0, E8, true);
+        else if (f.nv == E8) RN_FWD(true, 0, E8);
+        else if (f.stream) RN_FWD_NT(true, 0, 2 * E8, true);
         else RN_FWD(true, 0, 2 * E8);
     }
   } else {
@@ -981,9 +988,11 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
   }
 }
 #undef RN_FWD
+#undef RN_FWD_NT
 
-#define RN_BWD(TOK, L, NV)                                                                                                \
-  hipLaunchKernelGGL((rn_bwd_tile<T, TOK, L, NV, rn_vec<T>(TOK), MODE>), dim3(f.blocks), dim3(f.threads), 0, s, a)
+#define RN_BWD_NT(TOK, L, NV, NT)                                                                                         \
+  hipLaunchKernelGGL((rn_bwd_tile<T, TOK, L, NV, rn_vec<T>(TOK), NT, MODE>), dim3(f.blocks), dim3(f.threads), 0, s, a)
+#define RN_BWD(TOK, L, NV) RN_BWD_NT(TOK, L, NV, false)
 template <typename T, int MODE>
 void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
   constexpr int E8 = 8 / rn_vec<T>(true);
@@ -995,7 +1004,9 @@ void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
       case 32: RN_BWD(true, 32, E8); break;
       case 64: RN_BWD(true, 64, E8); break;
       default:
-        if (f.nv == E8) RN_BWD(true, 0, E8);
+        if (f.nv == E8 && f.stream) RN_BWD_NT(true, 0, E8, true);
+        else if (f.nv == E8) RN_BWD(true, 0, E8);
+        else if (f.stream) RN_BWD_NT(true, 0, 2 * E8, true);
         else RN_BWD(true, 0, 2 * E8);
     }
   } else {
@@ -1009,6 +1020,7 @@ void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
   }
 }
 #undef RN_BWD
+#undef RN_BWD_NT
 template <typename T>
 void launch_bwd(const RnArgs& a, const RnForm& f, int mode, bool params, hipStream_t s) {
   if (f.lanes < 0) {

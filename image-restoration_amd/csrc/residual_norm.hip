@@ -141,15 +141,22 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
     if (f.threads > most) f.lanes = -1;
     else a.tiles = (int)(((long)a.P + f.lanes * 4 - 1) / (f.lanes * 4));
   }
+  // Operands that the 256 MB cache cannot hold between their producer and this call are read past it, where a row is some
+  // kilobytes: tokens 2x8192x2048 fp32 forward 4.99 -> 6.24 TB/s, 4x4096x2048 bf16 backward 4.4 -> 4.9; smaller ones
+  // lose (8000x1000 fp32 6.0 -> 5.9, 2x4096x1024 bf16 5.0 -> 4.3), and so do narrow pieces of planar rows.
+  const int tensors = backward ? (a.pre ? 4 : 2) + (a.post || a.gate_kind ? 2 : 1) : a.pre ? 4 : 3;
+  f.stream = f.tok && f.lanes == 0 && image_bytes * a.B * tensors > 256l << 20;
   // Workers.  Workgroups of a kernel that loops over its tiles are best all resident at once (256 CUs, and a CU holds 8 waves
   // of the backward's 256 registers, 16 and more of the forward's); more and smaller ones only while they are small.  Tokens
   // 4x4096x2048 bf16 backward (256 threads): 256 / 512 / 1024 workgroups 143 / 94 / 108 us; 4x1066x3344 fp16: 512 threads
-  // 37 / 41 / 51 us; planar 13x153x21471 fp16 forward (320 threads): 512 / 1024 / 2048 114 / 141 / 132 us.  In the
-  // backward each also leaves a row of partial sums.
+  // 37 / 41 / 51 us; tokens 19061x2905 fp16 forward (384 threads): 512 / 768 / 1024 90 / 73 / 95 us; planar 13x153x21471
+  // fp16 forward (320 threads): 512 / 1024 / 2048 114 / 141 / 132 us.  In the backward each also leaves a row of partial
+  // sums.
   if (f.lanes < 0) a.tiles = (int)(((long)a.P + 63) / 64);
   long want = 256;
   if (f.lanes >= 0) {
     if (backward) want = 256 * std::max(1, 512 / f.threads);
+    else if (f.tok && f.lanes == 0 && f.threads >= 256) want = 256 * (1152 / f.threads);
     else want = f.threads <= 256 ? 2048 : f.threads <= 512 ? 512 : 256;
   }
   want *= per_block;
