@@ -35,7 +35,8 @@ enum { RN_Q_G1 = 0, RN_Q_G0 = 1, RN_Q_PRE_W = 2, RN_Q_PRE_B = 3, RN_Q_N = 4 };
 // Which kernel serves a call.  lanes: tokens - threads per token (4..64, several tokens per wave) or 0 (the whole
 // workgroup); planar - pixel lanes; -1: the sweep form.
 struct RnForm {
-  bool tok, stream;        // stream: operands larger than the caches, read past them
+  bool tok;
+  int stream;              // 1: operands larger than the caches are read past them, 2: outputs written past them too
   int lanes, nv, threads;
   unsigned blocks;
 };
@@ -66,7 +67,7 @@ template <> struct Elem<_Float16> {
 
 // VEC consecutive elements, read and written at the alignment of one element (rows of odd length, channel slices: the
 // memory instructions take any 2- or 4-byte address), `off` bytes into an image.
-// NT: read once and not kept in the caches.
+// NT: not kept in the caches.
 template <typename T, int VEC, bool NT> struct Pack {
   typedef T V __attribute__((ext_vector_type(VEC)));
   typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
@@ -77,14 +78,15 @@ template <typename T, int VEC, bool NT> struct Pack {
   }
   __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
 };
-template <typename T, int VEC>
+template <typename T, int VEC, bool NT = false>
 __device__ __forceinline__ void store_vec(char* image, unsigned off, const float* f) {
   typedef T V __attribute__((ext_vector_type(VEC)));
   typedef T VU __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
   V v;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) v[i] = (T)f[i];
-  *reinterpret_cast<VU*>(image + off) = v;
+  if (NT) __builtin_nontemporal_store(v, reinterpret_cast<VU*>(image + off));
+  else *reinterpret_cast<VU*>(image + off) = v;
 }
 // the last `own` of VEC values
 template <typename T, int VEC>
@@ -153,11 +155,11 @@ __device__ __forceinline__ float recip_sqrt(float x) {
 // none branches; the elements it then shares with its neighbour belong to the neighbour: they are left out of sums and
 // stores.  A thread without a channel repeats the last one and owns nothing.  Needs C >= VEC (tokens) or P >= VEC (planar),
 // and less than 2^32 bytes in an image.
-template <typename T, bool TOK, int L, int NV, int VEC, bool NT>
+template <typename T, bool TOK, int L, int NV, int VEC, int NT>
 struct Tile {
   static constexpr int NS = TOK ? 1 : VEC;       // statistics per thread: its token's, or one per pixel of its vector
   static constexpr int NP = TOK ? VEC : 1;       // parameters per vector
-  typedef Pack<T, VEC, NT> Vec;
+  typedef Pack<T, VEC, (NT > 0)> Vec;
   const RnArgs& a;
   float* red;                                    // LDS of two reductions
   int buf;
@@ -221,7 +223,7 @@ struct Tile {
     if (!edge(t)) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (own[j]) store_vec<T, VEC>(img, st + off[j], f[j]);
+        if (own[j]) store_vec<T, VEC, NT == 2>(img, st + off[j], f[j]);
     } else {
       const int px = own_pixels(t);
 #pragma unroll
@@ -321,7 +323,7 @@ struct Tile {
 
 // Forward.  Reads x and f once and writes y and n once; the next tile's loads are issued before this tile's reductions.
 // The branch's factors are folded: u = vh (gate w) + gate b.
-template <typename T, bool TOK, int L, int NV, int VEC, bool NT>
+template <typename T, bool TOK, int L, int NV, int VEC, int NT>
 __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_T16 : RN_T) void rn_fwd_tile(const RnArgs a) {
   typedef Tile<T, TOK, L, NV, VEC, NT> Ti;
   typedef typename Ti::Vec Vec;
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
 
 // Backward.  Every operand once; the parameter gradients accumulate in the registers of the threads that hold the
 // channel, over all of the worker's tiles, and are added up across lanes and waves once, at the end.
-template <typename T, bool TOK, int L, int NV, int VEC, bool NT, int MODE>
+template <typename T, bool TOK, int L, int NV, int VEC, int NT, int MODE>
 __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_bwd_tile(const RnArgs a) {
   typedef Tile<T, TOK, L, NV, VEC, NT> Ti;
   typedef typename Ti::Vec Vec;
@@ -957,7 +959,7 @@ unsigned sweep_blocks(bool tok, int B, int P) {
 
 #define RN_FWD_NT(TOK, L, NV, NT)                                                                                         \
   hipLaunchKernelGGL((rn_fwd_tile<T, TOK, L, NV, rn_vec<T>(TOK), NT>), dim3(f.blocks), dim3(f.threads), 0, s, a)
-#define RN_FWD(TOK, L, NV) RN_FWD_NT(TOK, L, NV, false)
+#define RN_FWD(TOK, L, NV) RN_FWD_NT(TOK, L, NV, 0)
 template <typename T>
 void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
   constexpr int E8 = 8 / rn_vec<T>(true);       // vectors for eight channels per thread
@@ -972,10 +974,15 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
       case 32: RN_FWD(true, 32, E8); break;
       case 64: RN_FWD(true, 64, E8); break;
       default:
-        if (f.nv == E8 && f.stream) RN_FWD_NT(true, 0, E8, true);
-        else if (f.nv == E8) RN_FWD(true, 0, E8);
-        else if (f.stream) RN_FWD_NT(true, 0, 2 * E8, true);
-        else RN_FWD(true, 0, 2 * E8);
+        if (f.nv == E8) {
+          if (f.stream == 2) RN_FWD_NT(true, 0, E8, 2);
+          else if (f.stream) RN_FWD_NT(true, 0, E8, 1);
+          else RN_FWD(true, 0, E8);
+        } else {
+          if (f.stream == 2) RN_FWD_NT(true, 0, 2 * E8, 2);
+          else if (f.stream) RN_FWD_NT(true, 0, 2 * E8, 1);
+          else RN_FWD(true, 0, 2 * E8);
+        }
     }
   } else {
     switch (f.lanes) {
@@ -992,7 +999,7 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
 
 #define RN_BWD_NT(TOK, L, NV, NT)                                                                                         \
   hipLaunchKernelGGL((rn_bwd_tile<T, TOK, L, NV, rn_vec<T>(TOK), NT, MODE>), dim3(f.blocks), dim3(f.threads), 0, s, a)
-#define RN_BWD(TOK, L, NV) RN_BWD_NT(TOK, L, NV, false)
+#define RN_BWD(TOK, L, NV) RN_BWD_NT(TOK, L, NV, 0)
 template <typename T, int MODE>
 void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
   constexpr int E8 = 8 / rn_vec<T>(true);
@@ -1004,9 +1011,9 @@ void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
       case 32: RN_BWD(true, 32, E8); break;
       case 64: RN_BWD(true, 64, E8); break;
       default:
-        if (f.nv == E8 && f.stream) RN_BWD_NT(true, 0, E8, true);
+        if (f.nv == E8 && f.stream) RN_BWD_NT(true, 0, E8, 1);
         else if (f.nv == E8) RN_BWD(true, 0, E8);
-        else if (f.stream) RN_BWD_NT(true, 0, 2 * E8, true);
+        else if (f.stream) RN_BWD_NT(true, 0, 2 * E8, 1);
         else RN_BWD(true, 0, 2 * E8);
     }
   } else {

@@ -144,8 +144,10 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
   // Operands that the 256 MB cache cannot hold between their producer and this call are read past it, where a row is some
   // kilobytes: tokens 2x8192x2048 fp32 forward 4.99 -> 6.24 TB/s, 4x4096x2048 bf16 backward 4.4 -> 4.9; smaller ones
   // lose (8000x1000 fp32 6.0 -> 5.9, 2x4096x1024 bf16 5.0 -> 4.3), and so do narrow pieces of planar rows.
+  // Outputs beyond it go past it too in the forward (8x4096x4096 bf16 5.0 -> 5.5 TB/s; below that 5.9 -> 5.3).
   const int tensors = backward ? (a.pre ? 4 : 2) + (a.post || a.gate_kind ? 2 : 1) : a.pre ? 4 : 3;
-  f.stream = f.tok && f.lanes == 0 && image_bytes * a.B * tensors > 256l << 20;
+  const long bytes = image_bytes * a.B, cache = 256l << 20;
+  f.stream = !f.tok || f.lanes != 0 || bytes * tensors <= cache ? 0 : !backward && bytes * (a.pre ? 2 : 1) > cache ? 2 : 1;
   // Workers.  Workgroups of a kernel that loops over its tiles are best all resident at once (256 CUs, and a CU holds 8 waves
   // of the backward's 256 registers, 16 and more of the forward's); more and smaller ones only while they are small.  Tokens
   // 4x4096x2048 bf16 backward (256 threads): 256 / 512 / 1024 workgroups 143 / 94 / 108 us; 4x1066x3344 fp16: 512 threads
