@@ -106,7 +106,8 @@ class AstTrainStep:
     def __init__(self, cfg: dict, state: Dict[str, np.ndarray], device: int = 0, lr: float = 2e-4,
                  betas=(0.9, 0.999), eps: float = 1e-8, use_grad_clip: bool = True, max_norm: float = 0.01,
                  loss_weight: float = 1.0, coupled: bool = True, adam_form: str = "jittor", process_group=None,
-                 drop_path_rate: Optional[float] = None, seed: int = 0, use_graph: bool = False):
+                 drop_path_rate: Optional[float] = None, seed: int = 0, use_graph: bool = False,
+                 fuse_residual_norm: bool = False):
         if cfg.get("token_mlp", "leff") != "frfn":
             raise NotImplementedError("AstTrainStep: only token_mlp='frfn' (the shipped AST configurations) is built")
         if not torch.cuda.is_available():
@@ -158,6 +159,9 @@ class AstTrainStep:
         self._stream = None
         # use_graph: optimize_parameters replays forward + backward as one captured hipGraph (from the second step on)
         self.use_graph = bool(use_graph)
+        # fuse_residual_norm: where an attention branch is under stochastic depth, its scaled sum with the shortcut and the
+        # norm of the MLP branch are one kernel, forward and backward (results differ in the last bits)
+        self.fuse_residual_norm = bool(fuse_residual_norm)
         self._graph, self._graph_key, self._graph_in, self._graph_out = None, None, None, None
         self._graph_generation = -1
         self._eager_shapes = set()       # input shapes that have run a step outside a capture (scratch is sized)
@@ -327,6 +331,22 @@ class AstTrainStep:
         check(self.L.jirf_train_scale_add(_vp(a.ptr if a else None), a.bs if a else 0, _vp(b.ptr), b.bs,
                                           _vp(scale.data_ptr()), _vp(y.ptr), y.bs, B, n_img, self._s()))
 
+    def residual_norm(self, x: V, br: V, scale: torch.Tensor, key: str, y: V, n: V, B, Cn, P) -> torch.Tensor:
+        """y = x + scale[b] * br and n = LayerNorm(y) in one pass; returns the statistics residual_norm_bwd reads."""
+        stats = torch.empty(4 * B * P, dtype=torch.float32, device=self.device)
+        check(self.L.jirf_train_residual_norm(x.ptr, x.bs, br.ptr, br.bs, 0, 0, 0, None, None, 0, None, scale.data_ptr(), 1,
+                                              self.P(key + ".weight"), self.P(key + ".bias"), 1e-5, y.ptr, y.bs, n.ptr, n.bs,
+                                              stats.data_ptr(), B, Cn, P, self._s()))
+        return stats
+
+    def residual_norm_bwd(self, dy: V, dn: V, y: V, stats: torch.Tensor, scale: torch.Tensor, key: str, dx: V, dbr: V, B, Cn, P):
+        work = torch.empty(int(self.L.jirf_train_residual_norm_bwd_work_floats(0, 0, 0, 0, 1, B, Cn, P)), dtype=torch.float32,
+                           device=self.device)
+        check(self.L.jirf_train_residual_norm_bwd(dy.ptr, dy.bs, dn.ptr, dn.bs, y.ptr, y.bs, None, 0, stats.data_ptr(), 0, 0, 0, None,
+                                                  None, 0, None, scale.data_ptr(), 1, self.P(key + ".weight"), dx.ptr, dx.bs,
+                                                  dbr.ptr, dbr.bs, None, None, None, self.G(key + ".weight"), self.G(key + ".bias"),
+                                                  0, work.data_ptr(), B, Cn, P, self._s()))
+
     # ---- one TransformerBlock (ast_arch.py:768-842) -------------------------------------------------------------
     def _blocks(self):
         out = []
@@ -362,6 +382,8 @@ class AstTrainStep:
         dc = Cn // 4
         sv = dict(x=x)
         cur = x
+        cat = self.buf(B, Cn, P)                       # norm2(x), then its first C/4 channels replaced by the 3x3's output
+        normed = False
         if bl["att"]:
             a = n + ".attn"
             n1 = self.buf(B, Cn, P)
@@ -381,12 +403,16 @@ class AstTrainStep:
             else:                                          # x + drop_path(branch)
                 br = self.buf(B, Cn, P)
                 self.conv(ao, self.P(a + ".proj.weight"), W_FWD, self.P(a + ".proj.bias"), None, br, B, Cn, Cn, H, W)
-                self.scale_add(x, br, sa, x1, B, Cn * P)
+                if self.fuse_residual_norm:
+                    sv["join"] = self.residual_norm(x, br, sa, n + ".norm2", x1, cat, B, Cn, P)
+                    normed = True
+                else:
+                    self.scale_add(x, br, sa, x1, B, Cn * P)
             sv.update(n1=n1, qkv=qkv, ao=ao, x1=x1, s_attn=sa)
             cur = x1
         m = n + ".mlp"
-        cat = self.buf(B, Cn, P)                       # norm2(x), then its first C/4 channels replaced by the 3x3's output
-        self.layernorm(cur, n + ".norm2", cat, B, Cn, P)
+        if not normed:
+            self.layernorm(cur, n + ".norm2", cat, B, Cn, P)
         first = self.buf(B, dc, P)
         self.add(cat, None, first, B, dc * P)
         self.conv(first, self.P(m + ".partial_conv3.weight"), W_FWD, None, None, cat, B, dc, dc, H, W, 3, 1, 1)
@@ -447,12 +473,16 @@ class AstTrainStep:
         self.add(dfirst, None, dcat, B, dc * P)
         # norm2 and the shortcut around the MLP
         dcur = self.buf(B, Cn, P)
-        self.layernorm_bwd(sv["cur"], dcat, n + ".norm2", dout, dcur, B, Cn, P)
+        dbr = dcur
+        if "join" in sv:
+            dbr = self.buf(B, Cn, P)
+            self.residual_norm_bwd(dout, dcat, sv["cur"], sv["join"], sv["s_attn"], n + ".norm2", dcur, dbr, B, Cn, P)
+        else:
+            self.layernorm_bwd(sv["cur"], dcat, n + ".norm2", dout, dcur, B, Cn, P)
         if not bl["att"]:
             return dcur
         a = n + ".attn"
-        dbr = dcur
-        if sv.get("s_attn") is not None:
+        if sv.get("s_attn") is not None and "join" not in sv:
             dbr = self.buf(B, Cn, P)
             self.scale_add(None, dcur, sv["s_attn"], dbr, B, Cn * P)
         self.conv_dw(dbr, sv["ao"], self.G(a + ".proj.weight"), self.G(a + ".proj.bias"), B, Cn, Cn, H, W, H, W)

@@ -10,7 +10,6 @@ any.  There is no CPU path and no autograd graph: the backward is called by name
 from __future__ import annotations
 
 import ctypes as C
-import functools
 import math
 from typing import NamedTuple, Optional, Sequence, Tuple
 
@@ -56,9 +55,10 @@ def _bs(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
         raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(like.shape)} {like.dtype} on {like.device}")
     if t.is_contiguous():
         return 0
-    if not t[0].is_contiguous():
-        raise ValueError(f"{name}: each image has to be contiguous (strides {t.stride()})")
-    return t.stride(0)
+    bs = t.stride(0)
+    if not t[0].is_contiguous() or bs < t[0].numel():
+        raise ValueError(f"{name}: each image has to be contiguous and apart from the others (strides {t.stride()})")
+    return bs
 
 
 def _param(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> int:
@@ -89,22 +89,10 @@ def _gate(gate: Optional[torch.Tensor], B: int, Cn: int, like: torch.Tensor):
     return 2, _param("gate", gate, (B, Cn), like)
 
 
-def _on_device(fn):
-    """Runs fn with the device of its first tensor argument current (a switch only where it is not already)."""
-    def call(*args, **kw):
-        t = next((a for a in (*args, *kw.values()) if isinstance(a, torch.Tensor)), None)
-        if t is None or not t.is_cuda or t.get_device() == torch.cuda.current_device():
-            return fn(*args, **kw)
-        with torch.cuda.device(t.device):
-            return fn(*args, **kw)
-    return functools.wraps(fn)(call)
-
-
 def _new(x: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
-@_on_device
 def residual_norm(x: torch.Tensor, branch: torch.Tensor, *, post: Optional[Norm] = None, gate: Optional[torch.Tensor] = None,
                   scale: Optional[torch.Tensor] = None, pre: Optional[Norm] = None, layout: str = "planar", eps: float = 1e-5,
                   save_stats: bool = False, out: Optional[torch.Tensor] = None,
@@ -117,6 +105,10 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, *, post: Optional[Norm]
     save_stats: keep what residual_norm_bwd needs ([4, B, P] float32).  out, norm_out: where y and n go (out may be x,
     norm_out may be branch)."""
     B, Cn, P = _sizes(x, layout)
+    if x.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return residual_norm(x, branch, post=post, gate=gate, scale=scale, pre=pre, layout=layout, eps=eps,
+                                 save_stats=save_stats, out=out, norm_out=norm_out)
     fb = _bs("branch", branch, x)
     k0, w0, b0 = _norm("post", post, Cn, x)
     k1, w1, b1 = _norm("pre", pre, Cn, x)
@@ -135,7 +127,6 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, *, post: Optional[Norm]
     return ResidualNorm(y, n, stats)
 
 
-@_on_device
 def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y: Optional[torch.Tensor],
                       branch: Optional[torch.Tensor], stats: Optional[torch.Tensor], *, post: Optional[Norm] = None,
                       gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, pre: Optional[Norm] = None,
@@ -147,6 +138,9 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
     if like is None:
         raise ValueError("residual_norm_bwd: dy or dn is needed")
     B, Cn, P = _sizes(like, layout)
+    if like.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(like.device):
+            return residual_norm_bwd(dy, dn, y, branch, stats, post=post, gate=gate, scale=scale, pre=pre, layout=layout)
     k0, w0, b0 = _norm("post", post, Cn, like)
     k1, w1, b1 = _norm("pre", pre, Cn, like)
     gk, gp = _gate(gate, B, Cn, like)

@@ -111,3 +111,31 @@ def test_python_layer_refuses():
         T.GradientClip([x])
     with pytest.raises(ValueError, match="2 tensors, 1 outputs"):
         T.GradientClip([x, x], out=[x])
+
+
+def test_python_layer_refuses_strides():
+    """Images that overlap (an expanded batch), or are not contiguous themselves."""
+    one = torch.zeros(1, 8, 6)
+    like = torch.zeros(3, 8, 6)
+    assert T._bs("x", like, like) == 0 and T._bs("x", torch.zeros(3, 16, 6)[:, :8], like) == 96
+    for bad in (one.expand(3, 8, 6), torch.zeros(3, 6, 8).transpose(1, 2), torch.zeros(3, 8, 12)[..., ::2],
+                torch.zeros(100).as_strided((3, 8, 6), (8, 6, 1))):
+        with pytest.raises(ValueError, match="contiguous"):
+            T._bs("x", bad, like)
+    for bad in (torch.zeros(3, 8, 7), torch.zeros(3, 8, 6, dtype=torch.float16)):
+        with pytest.raises(ValueError, match="expected"):
+            T._bs("x", bad, like)
+
+
+def test_python_layer_refuses_parameters():
+    like = torch.zeros(3, 8, 6)
+    good = torch.zeros(8)
+    assert T._norm("pre", ("WithBias", good, good), 8, like)[0] == 1 and T._norm("pre", ("RMS", good, None), 8, like)[0] == 3
+    assert T._gate(good, 3, 8, like)[0] == 1 and T._gate(torch.zeros(3, 8), 3, 8, like)[0] == 2 and T._gate(None, 3, 8, like) == (0, None)
+    for spec in ((4, good, None), ("LayerNorm", good, None), ("RMS", good, good), (2, good, good), (1, torch.zeros(7), None),
+                 (1, good.half(), None), (1, good, torch.zeros(9)), (3, torch.zeros(16)[::2], None)):
+        with pytest.raises(ValueError):
+            T._norm("pre", spec, 8, like)
+    for gate in (torch.zeros(6), torch.zeros(2, 8), torch.zeros(3, 8, 6), good.bfloat16()):
+        with pytest.raises(ValueError):
+            T._gate(gate, 3, 8, like)
