@@ -328,7 +328,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
   typedef Tile<T, TOK, L, NV, VEC, NT> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
-  __shared__ __attribute__((aligned(16))) float lds[Ti::RED];
+  __shared__ __attribute__((aligned(32))) float lds[Ti::RED];
   Ti ti(a, lds);
   int b0, b1, t0;
   ti.range(ti.worker(), b0, b1, t0);
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_bwd_tile(const
   constexpr int EW = NV * NP;                                  // channels of a thread
   // the next tile's operands are fetched ahead where the registers (256 per thread) have room for two tiles
   constexpr bool PF = !(BR && NV * VEC == 16 && (sizeof(T) == 4 || IG));
-  __shared__ __attribute__((aligned(16))) float lds[Ti::RED];
+  __shared__ __attribute__((aligned(32))) float lds[Ti::RED];
   __shared__ float wsum[TOK && L ? RN_LANE_T / 64 * L * EW : 1];
   Ti ti(a, lds);
   int b0, b1, t0;
@@ -566,7 +566,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_bwd_tile(const
 #pragma unroll
           for (int i = 0; i < VEC; ++i) d[j][i] = dy[j].at(i);
       }
-      ti.store(a.dx, a.dx_bs, b, t, d);
+      if (a.dx) ti.store(a.dx, a.dx_bs, b, t, d);
       if (!BR) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -819,7 +819,7 @@ __global__ __launch_bounds__(256) void rn_bwd_sweep(const RnArgs a) {
     const T* dn = a.pre ? static_cast<const T*>(a.dn) + b * a.dn_bs + o : nullptr;
     const T* y = a.pre ? static_cast<const T*>(a.y_in) + b * a.yi_bs + o : nullptr;
     const T* f = a.post ? static_cast<const T*>(a.f) + b * a.f_bs + o : nullptr;
-    T* dx = static_cast<T*>(a.dx) + b * a.dx_bs + o;
+    T* dx = a.dx ? static_cast<T*>(a.dx) + b * a.dx_bs + o : nullptr;
     T* df = static_cast<T*>(a.df) + b * a.df_bs + o;
     const float* gate = a.gate_kind == 2 ? a.gate + b * a.C : a.gate;
     RowBwd r{};
@@ -865,7 +865,7 @@ __global__ __launch_bounds__(256) void rn_bwd_sweep(const RnArgs a) {
         const float d = dyt(c);
         float du = d * (a.gate_kind ? r.s * gate[c] : r.s);
         if (a.post) du = r.rs0 * (du * a.post_w[c] - t1 - (Elem<T>::ld(f + c * a.cs) - r.mu0) * r.rs0 * t2);
-        Elem<T>::st(dx + c * a.cs, d);
+        if (dx) Elem<T>::st(dx + c * a.cs, d);
         Elem<T>::st(df + c * a.cs, du);
       }
   }

@@ -342,7 +342,7 @@ int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, lon
   return guarded_r([&] {
     const char* who = "residual_norm_bwd";
     check_common(who, dtype, layout, post_kind, post_w, gate_kind, gate, pre_kind, pre_w, B, C, P);
-    JIRF_REQUIRE(dx && df && (dy || pre_kind), JIRF_EINVAL, "%s: null activation gradient", who);
+    JIRF_REQUIRE((dx || !pre_kind) && df && (dy || pre_kind), JIRF_EINVAL, "%s: null activation gradient", who);
     JIRF_REQUIRE(!pre_kind || (dn && y), JIRF_EINVAL, "%s: the norm before the next block needs dn and y", who);
     JIRF_REQUIRE(!(post_kind || gate_kind) || f, JIRF_EINVAL, "%s: a norm or gate on the branch needs f", who);
     JIRF_REQUIRE(!(post_kind || pre_kind) || stats, JIRF_EINVAL, "%s: a norm needs the forward's statistics", who);

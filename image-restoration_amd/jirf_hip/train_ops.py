@@ -133,7 +133,8 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
                       layout: str = "planar") -> dict:
     """Gradients of residual_norm: {"dx", "dbranch", "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b"}, None where
     there is no such input.  dy: gradient of y (None: zero), dn: gradient of n; y, stats: the forward's; branch: the
-    forward's input (needed with a post norm or a gate)."""
+    forward's input (needed with a post norm or a gate).  Without a pre norm dx is dy itself, not a copy, and so is
+    dbranch where the branch has no norm, gate or scale either."""
     like = dy if dy is not None else dn
     if like is None:
         raise ValueError("residual_norm_bwd: dy or dn is needed")
@@ -155,9 +156,11 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
     if dy is None and not k1:
         raise ValueError("residual_norm_bwd: without a pre norm dy is needed")
     st = _param("stats", stats, (4, B, P), like) if k0 or k1 else None
+    if not (k0 or gk or k1 or sp):
+        return dict(dx=dy, dbranch=dy, dgate=None, dpost_w=None, dpost_b=None, dpre_w=None, dpre_b=None)
     dtype, lay = _DTYPES[like.dtype], LAYOUTS[layout]
     L = lib()
-    dx, df = _new(like), _new(like)
+    dx, df = _new(like) if k1 else dy, _new(like)
     # the [C] gradients are rows of one tensor
     rows = [None] * 5
     wanted = [i for i, on in enumerate((k0, b0 is not None, gk == 1, k1, b1 is not None)) if on]
@@ -173,7 +176,7 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
         None if dy is None else dy.data_ptr(), 0 if dy is None else _bs("dy", dy, like), dn.data_ptr() if k1 else None,
         _bs("dn", dn, like) if k1 else 0, y.data_ptr() if k1 else None, _bs("y", y, like) if k1 else 0,
         branch.data_ptr() if use_f else None, _bs("branch", branch, like) if use_f else 0, st, dtype, lay, k0, w0, b0, gk, gp, sp,
-        k1, w1, dx.data_ptr(), 0, df.data_ptr(), 0, p[0], p[1], p[2], p[3], p[4], 0, work.data_ptr(), B, Cn, P,
+        k1, w1, dx.data_ptr() if k1 else None, 0, df.data_ptr(), 0, p[0], p[1], p[2], p[3], p[4], 0, work.data_ptr(), B, Cn, P,
         _raw_stream(like.get_device())))
     return dict(dx=dx, dbranch=df, dgate=rows[2], dpost_w=rows[0], dpost_b=rows[1], dpre_w=rows[3], dpre_b=rows[4])
 

@@ -461,7 +461,7 @@ int jirf_train_residual_norm(const void* x, long x_bs, const void* f, long f_bs,
                              long n_bs, float* stats, int B, int C, int P, void* stream);
 /* Its backward.  dy (or NULL: zero) is the gradient arriving over the residual stream, dn that of n; y and stats are the
  * forward's, f its branch input (NULL where neither norm nor gate sits on the branch; dn, y NULL without N_pre).
- *     dx = dy + dN_pre(dn),   df = dN_post(scale * gate * dx)
+ *     dx = dy + dN_pre(dn),   df = dN_post(scale * gate * dx)     (without N_pre dx is dy: it may be NULL, not written)
  * and the parameter gradients dpost_w, dpost_b, dpre_w, dpre_b [C], dgate [C] or [B][C], each NULL when not wanted,
  * accumulate != 0 adds to them.  No gradient for scale (it is drawn, not learned).  work: DEVICE memory of
  * jirf_train_residual_norm_bwd_work_floats() floats owned by the caller, needed only during the call (calls that

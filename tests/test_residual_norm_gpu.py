@@ -376,3 +376,23 @@ def test_offsets_past_32_bits():
     small = T.residual_norm(tail[None], (-0.5 * tail)[None], pre=(3, w, None))
     assert torch.equal(r.y[1, :, P - 70:], small.y[0]) and torch.equal(r.n[1, :, P - 70:], small.n[0])
     assert not r.y[0].any() and not r.n[1, :, : P - 70].any()
+
+
+@pytest.mark.parametrize("layout,C", [("planar", 48), ("planar", 2100), ("tokens", 200), ("tokens", 9000)])
+def test_without_a_pre_norm_dx_is_dy(layout, C):
+    """The stream's gradient passes through unchanged and uncopied; written where the caller of the C entry asks for it."""
+    B, P = 2, 30
+    d = make(layout, F32, B, C, P, 0, 1, 0, True, seed=19)
+    kw = dict(gate=d["gate"], scale=d["scale"], layout=layout)
+    g = T.residual_norm_bwd(d["dy"], None, None, d["f"], None, **kw)
+    assert g["dx"] is d["dy"]
+    assert all(T.residual_norm_bwd(d["dy"], None, None, None, None, layout=layout)[k] is d["dy"] for k in ("dx", "dbranch"))
+    lay = T.LAYOUTS[layout]
+    work = torch.empty(jirf_hip.lib().jirf_train_residual_norm_bwd_work_floats(0, lay, 0, 1, 0, B, C, P), device="cuda")
+    for want in (False, True):
+        dx, df, dg = torch.full_like(d["dy"], 7.0), torch.empty_like(d["dy"]), torch.empty(C, device="cuda")
+        call("jirf_train_residual_norm_bwd", ptr(d["dy"]), 0, None, 0, None, 0, ptr(d["f"]), 0, None, 0, lay, 0, None, None, 1,
+             ptr(d["gate"]), ptr(d["scale"]), 0, None, ptr(dx) if want else None, 0, ptr(df), 0, None, None, ptr(dg), None, None, 0,
+             ptr(work), B, C, P, stream())
+        assert torch.equal(df, g["dbranch"]) and torch.equal(dg, g["dgate"])
+        assert torch.equal(dx, d["dy"]) if want else (dx == 7).all()

@@ -44,7 +44,7 @@ def test_forward_refuses(kw):
 
 
 @pytest.mark.parametrize("kw", BAD_COMMON + [
-    dict(dx=None), dict(df=None), dict(dy=None), dict(pre=1, pre_w=A, y=B_, stats=B_, work=A), dict(pre=1, pre_w=A, dn=B_, stats=B_, work=A),
+    dict(dx=None, pre=1, pre_w=A, dn=B_, y=B_, stats=B_, work=A), dict(df=None), dict(dy=None), dict(pre=1, pre_w=A, y=B_, stats=B_, work=A), dict(pre=1, pre_w=A, dn=B_, stats=B_, work=A),
     dict(pre=1, pre_w=A, dn=B_, y=B_, work=A), dict(pre=1, dn=B_, y=B_, stats=B_, work=A), dict(post=1, post_w=A, stats=B_, work=A),
     dict(gate_kind=1, gate=A, work=A), dict(post=2, post_w=A, f=B_, work=A), dict(dpost_w=A, work=A), dict(dgate=A, work=A),
     dict(dpre_w=A, work=A), dict(dpre_b=A, work=A), dict(post=2, post_w=A, f=B_, stats=B_, dpost_b=A, work=A),
