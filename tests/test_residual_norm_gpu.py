@@ -396,3 +396,90 @@ def test_without_a_pre_norm_dx_is_dy(layout, C):
              ptr(work), B, C, P, stream())
         assert torch.equal(df, g["dbranch"]) and torch.equal(dg, g["dgate"])
         assert torch.equal(dx, d["dy"]) if want else (dx == 7).all()
+
+
+@pytest.mark.parametrize("layout", ["planar", "tokens"])
+def test_an_image_past_32_bits(layout):
+    """4.6 GB in one image: every byte offset past 2^32, forward and backward; all but the last pixels are zero, so the
+    parameter gradients are those of the last pixels alone (summed in another order: the bound of each side)."""
+    C, P, n = 64, 18_000_064, 70
+    shape = (1, C, P) if layout == "planar" else (1, P, C)
+    last = (lambda t: t[..., P - n:]) if layout == "planar" else (lambda t: t[:, P - n:])          # noqa: E731
+    g = gen(20)
+    small = {k: torch.randn((1, C, n) if layout == "planar" else (1, n, C), generator=g).cuda() for k in ("x", "f", "dy", "dn")}
+    big = {}
+    for k, t in small.items():
+        big[k] = torch.zeros(shape, device="cuda")
+        last(big[k]).copy_(t)
+    w, gate = (1 + 0.2 * torch.randn(C, generator=g)).cuda(), torch.randn(C, generator=g).cuda()
+    kw = dict(post=(3, w, None), gate=gate, pre=(1, w, None), layout=layout)
+    R1 = T.residual_norm(big["x"], big["f"], save_stats=True, **kw)
+    r = T.residual_norm(small["x"], small["f"], save_stats=True, **kw)
+    K = R.chain(C, layout)
+    want = R.forward(small["x"], small["f"], kw["post"], gate, None, kw["pre"], layout, EPS)
+    for got, name in ((last(R1.y), "y"), (last(R1.n), "n")):
+        R.check(name, got, want[name], K, layout)
+    assert not R1.y.flatten()[: 10_000_000].any()
+    d = T.residual_norm_bwd(big["dy"], big["dn"], R1.y, big["f"], R1.stats, **kw)
+    want = R.backward(small["dy"], small["dn"], r.y, small["f"], r.stats, kw["post"], gate, None, kw["pre"], layout, EPS)
+    for k in ("dx", "dbranch"):
+        R.check(k, last(d[k]), want[k], 4 * K + 80, layout)
+    for k in ("dgate", "dpost_w", "dpre_w"):
+        R.check(k, d[k], want[k], 4 * K + 80)
+
+
+@pytest.mark.parametrize("layout,dtype,C,P", [("planar", F32, 5, 9), ("planar", BF16, 70, 131), ("tokens", F32, 9, 6),
+                                              ("tokens", BF16, 9, 6), ("tokens", F16, 523, 6), ("tokens", F32, 2051, 3)])
+def test_an_infinity_where_vectors_meet(layout, dtype, C, P):
+    """Near a ragged end two threads hold the same element, and one of them owns it: an infinity there counts once (inf, not
+    inf - inf or inf * 0) and leaves every other channel's gradient as it is."""
+    d = make(layout, dtype, 2, C, P, 0, 1, 0, False, seed=21)
+    kw = dict(gate=d["gate"], layout=layout)
+    d["dy"].abs_().add_(0.5)
+    clean = T.residual_norm_bwd(d["dy"], None, None, d["f"], None, **kw)["dgate"]
+    for back in range(1, 9):
+        f = d["f"].clone()
+        c, p = (C // 2, P - back) if layout == "planar" else (C - back, P // 2)
+        (f[1, c] if layout == "planar" else f[1, :, c])[p] = float("inf")
+        dg = T.residual_norm_bwd(d["dy"], None, None, f, None, **kw)["dgate"]
+        assert dg[c] == float("inf"), (back, float(dg[c]))
+        others = torch.arange(C, device="cuda") != c
+        assert torch.equal(dg[others], clean[others])
+        # a gradient dn of infinity: the same pattern of infinities and NaN as the formula gives
+        w = (1 + 0.1 * torch.arange(C, device="cuda") / C).float()
+        r = T.residual_norm(d["x"], d["f"], pre=(3, w, None), layout=layout, save_stats=True)
+        dn = d["dn"].clone()
+        (dn[1, c] if layout == "planar" else dn[1, :, c])[p] = float("inf")
+        g = T.residual_norm_bwd(d["dy"], dn, r.y, None, r.stats, pre=(3, w, None), layout=layout)
+        want = R.backward(d["dy"], dn, r.y, None, r.stats, None, None, None, (3, w, None), layout, EPS)
+        for k in ("dx", "dpre_w"):
+            got, ref = (R.tokens_last(g[k], layout) if k == "dx" else R.host(g[k])), want[k][0]
+            assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(torch.isinf(got), torch.isinf(ref)), (back, k)
+
+
+@pytest.mark.parametrize("dtype,C,P", [(BF16, 2048, 34000), (F32, 2051, 17000), (F16, 4100, 17000), (BF16, 4096, 33000)])
+def test_calls_larger_than_the_cache(dtype, C, P):
+    """Token rows whose operands (and, in the last case, outputs) are streamed past the caches: bit for bit what shorter
+    calls give row by row, and parameter gradients equal to the shorter calls' sum (each within its bound: the sums of
+    absolute terms at 32-bit roundings)."""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")                        # noqa: E731
+    x, f, dy, dn = (rnd(1, P, C).to(dtype) for _ in range(4))
+    w, gate = 1 + 0.2 * rnd(C), rnd(C)
+    kw = dict(post=(3, w, None), gate=gate, pre=(1, w, None), layout="tokens")
+    big = T.residual_norm(x, f, save_stats=True, **kw)
+    gb = T.residual_norm_bwd(dy, dn, big.y, f, big.stats, **kw)
+    cut, sums, mags = 4000, {}, {}
+    for p in range(0, P, cut):
+        s = slice(p, min(P, p + cut))
+        part = [t[:, s].contiguous() for t in (x, f, dy, dn)]
+        r = T.residual_norm(part[0], part[1], save_stats=True, **kw)
+        assert torch.equal(r.y, big.y[:, s]) and torch.equal(r.n, big.n[:, s]) and torch.equal(r.stats, big.stats[:, :, s])
+        d = T.residual_norm_bwd(part[2], part[3], r.y, part[1], r.stats, **kw)
+        assert torch.equal(d["dx"], gb["dx"][:, s]) and torch.equal(d["dbranch"], gb["dbranch"][:, s])
+        for k in ("dgate", "dpost_w", "dpre_w"):
+            sums[k] = sums.get(k, 0) + d[k].double()
+    # |terms| <= |dn| |vh| and so on are of order one each, so the sum of their magnitudes is at most about P; a worker adds
+    # at most P / 256 rows in 32 bits
+    for k, v in sums.items():
+        assert (gb[k].double() - v).abs().max() <= (P / 256 + 60) * 2.0 ** -24 * 8 * P, k
