@@ -33,25 +33,28 @@ class ResidualNorm(NamedTuple):
 
 
 def _sizes(x: torch.Tensor, layout: str):
-    if layout not in LAYOUTS:
+    """B, C, P, layout tag, dtype tag"""
+    lay = LAYOUTS.get(layout)
+    if lay is None:
         raise ValueError(f"layout {layout!r}: 'planar' ([B, C, ...]) or 'tokens' ([B, P, C])")
     if not x.is_cuda:
         raise ValueError("residual_norm needs GPU tensors: there is no CPU path")
-    if x.dtype not in _DTYPES:
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None:
         raise ValueError(f"dtype {x.dtype}: only float32, bfloat16 and float16")
     shape, n = x.shape, x.numel()
-    if len(shape) < 3 or (layout == "tokens" and len(shape) != 3):
+    if len(shape) < 3 or (lay and len(shape) != 3):
         raise ValueError(f"{layout} activations are [B, C, ...] / [B, P, C], got shape {tuple(shape)}")
     if n == 0:
         raise ValueError(f"empty activation {tuple(shape)}")
-    if layout == "planar":
-        return shape[0], shape[1], n // (shape[0] * shape[1])
-    return shape[0], shape[2], shape[1]
+    if lay:
+        return shape[0], shape[2], shape[1], lay, dtype
+    return shape[0], shape[1], n // (shape[0] * shape[1]), lay, dtype
 
 
 def _bs(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
     """Batch stride (0: dense) of an activation that has to match `like`."""
-    if t is not like and (t.shape != like.shape or t.dtype != like.dtype or t.get_device() != like.get_device()):
+    if t is not like and (t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(like.shape)} {like.dtype} on {like.device}")
     if t.is_contiguous():
         return 0
@@ -62,7 +65,7 @@ def _bs(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
 
 
 def _param(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> int:
-    if t.shape != shape or t.dtype != torch.float32 or t.get_device() != like.get_device() or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.shape != shape or t.get_device() != like.get_device() or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous float32 tensor {shape} on {like.device} is needed, got {tuple(t.shape)} {t.dtype} "
                          f"on {t.device}")
     return t.data_ptr()
@@ -73,12 +76,14 @@ def _norm(name: str, spec: Optional[Norm], Cn: int, like: torch.Tensor):
     if spec is None:
         return 0, None, None
     kind, w, b = spec
-    if kind not in NORM_KINDS:
+    k = NORM_KINDS.get(kind)
+    if k is None:
         raise ValueError(f"{name}: norm kind {kind!r}, one of {list(NORM_KINDS)}")
-    kind = NORM_KINDS[kind]
-    if b is not None and kind != 1:
+    if b is None:
+        return k, _param(name, w, (Cn,), like), None
+    if k != 1:
         raise ValueError(f"{name}: only the WithBias norm takes a bias")
-    return kind, _param(name + " weight", w, (Cn,), like), None if b is None else _param(name + " bias", b, (Cn,), like)
+    return k, _param(name, w, (Cn,), like), _param(name, b, (Cn,), like)
 
 
 def _gate(gate: Optional[torch.Tensor], B: int, Cn: int, like: torch.Tensor):
@@ -89,8 +94,8 @@ def _gate(gate: Optional[torch.Tensor], B: int, Cn: int, like: torch.Tensor):
     return 2, _param("gate", gate, (B, Cn), like)
 
 
-def _new(x: torch.Tensor) -> torch.Tensor:
-    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+def _new(x: torch.Tensor, dense: bool) -> torch.Tensor:
+    return torch.empty_like(x) if dense else x.new_empty(x.shape)
 
 
 def residual_norm(x: torch.Tensor, branch: torch.Tensor, *, post: Optional[Norm] = None, gate: Optional[torch.Tensor] = None,
@@ -104,26 +109,27 @@ def residual_norm(x: torch.Tensor, branch: torch.Tensor, *, post: Optional[Norm]
     or None.  gate: [C], [B, C] or None.  scale: [B] (a sample's DropPath factor) or None.  Parameters are float32.
     save_stats: keep what residual_norm_bwd needs ([4, B, P] float32).  out, norm_out: where y and n go (out may be x,
     norm_out may be branch)."""
-    B, Cn, P = _sizes(x, layout)
-    if x.get_device() != torch.cuda.current_device():
+    B, Cn, P, lay, dtype = _sizes(x, layout)
+    index = x.get_device()
+    if index != torch.cuda.current_device():
         with torch.cuda.device(x.device):
             return residual_norm(x, branch, post=post, gate=gate, scale=scale, pre=pre, layout=layout, eps=eps,
                                  save_stats=save_stats, out=out, norm_out=norm_out)
-    fb = _bs("branch", branch, x)
+    xb, fb = _bs("x", x, x), _bs("branch", branch, x)
     k0, w0, b0 = _norm("post", post, Cn, x)
     k1, w1, b1 = _norm("pre", pre, Cn, x)
     gk, gp = _gate(gate, B, Cn, x)
     sp = None if scale is None else _param("scale", scale, (B,), x)
     if norm_out is not None and not k1:
         raise ValueError("norm_out without a pre norm")
-    y = _new(x) if out is None else out
-    n = (_new(x) if norm_out is None else norm_out) if k1 else None
+    y = _new(x, xb == 0) if out is None else out
+    n = (_new(x, xb == 0) if norm_out is None else norm_out) if k1 else None
     stats = x.new_empty((4, B, P), dtype=torch.float32) if save_stats else None
     check(lib().jirf_train_residual_norm(
-        x.data_ptr(), _bs("x", x, x), branch.data_ptr(), fb, _DTYPES[x.dtype], LAYOUTS[layout], k0, w0, b0, gk, gp, sp, k1, w1,
+        x.data_ptr(), xb, branch.data_ptr(), fb, dtype, lay, k0, w0, b0, gk, gp, sp, k1, w1,
         b1, eps, y.data_ptr(), 0 if out is None else _bs("out", y, x), n.data_ptr() if k1 else None,
         0 if norm_out is None else _bs("norm_out", n, x), stats.data_ptr() if save_stats else None, B, Cn, P,
-        _raw_stream(x.get_device())))
+        _raw_stream(index)))
     return ResidualNorm(y, n, stats)
 
 
@@ -138,8 +144,9 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
     like = dy if dy is not None else dn
     if like is None:
         raise ValueError("residual_norm_bwd: dy or dn is needed")
-    B, Cn, P = _sizes(like, layout)
-    if like.get_device() != torch.cuda.current_device():
+    B, Cn, P, lay, dtype = _sizes(like, layout)
+    index = like.get_device()
+    if index != torch.cuda.current_device():
         with torch.cuda.device(like.device):
             return residual_norm_bwd(dy, dn, y, branch, stats, post=post, gate=gate, scale=scale, pre=pre, layout=layout)
     k0, w0, b0 = _norm("post", post, Cn, like)
@@ -158,9 +165,9 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
     st = _param("stats", stats, (4, B, P), like) if k0 or k1 else None
     if not (k0 or gk or k1 or sp):
         return dict(dx=dy, dbranch=dy, dgate=None, dpost_w=None, dpost_b=None, dpre_w=None, dpre_b=None)
-    dtype, lay = _DTYPES[like.dtype], LAYOUTS[layout]
     L = lib()
-    dx, df = _new(like) if k1 else dy, _new(like)
+    dense = like.is_contiguous()
+    dx, df = _new(like, dense) if k1 else dy, _new(like, dense)
     # the [C] gradients are rows of one tensor
     rows = [None] * 5
     wanted = [i for i, on in enumerate((k0, b0 is not None, gk == 1, k1, b1 is not None)) if on]
@@ -177,7 +184,7 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
         _bs("dn", dn, like) if k1 else 0, y.data_ptr() if k1 else None, _bs("y", y, like) if k1 else 0,
         branch.data_ptr() if use_f else None, _bs("branch", branch, like) if use_f else 0, st, dtype, lay, k0, w0, b0, gk, gp, sp,
         k1, w1, dx.data_ptr() if k1 else None, 0, df.data_ptr(), 0, p[0], p[1], p[2], p[3], p[4], 0, work.data_ptr(), B, Cn, P,
-        _raw_stream(like.get_device())))
+        _raw_stream(index)))
     return dict(dx=dx, dbranch=df, dgate=rows[2], dpost_w=rows[0], dpost_b=rows[1], dpre_w=rows[3], dpre_b=rows[4])
 
 
