@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <cmath>
 #include <memory>
+#include <type_traits>
 #include <vector>
 
 #include "runtime.h"
@@ -36,14 +37,11 @@ struct ClipChunk {
   unsigned types;         // source type | destination type << 8
 };
 
-// Eight consecutive elements, 16 bytes per access, at the alignment of one element (a tensor packed tight between others
-// starts anywhere; the memory instructions take any 4- or 2-byte address).
-typedef unsigned u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
+// Accesses of 8 and 16 bytes at the alignment of one element: the memory instructions take any 2- or 4-byte address.
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 // A chunk's addresses come out of memory: said to be device memory here, or every access would take the slower flat path.
 template <typename P>
@@ -55,70 +53,67 @@ __device__ __forceinline__ __attribute__((address_space(1))) P* dev(void* p, siz
   return reinterpret_cast<__attribute__((address_space(1))) P*>(reinterpret_cast<uintptr_t>(p) + byte);
 }
 
-template <int TY>
-struct Raw {              // eight elements as loaded
-  u32x4 a, b;             // b: fp32 only
+// E consecutive elements (4 or 8) as loaded - 8 or 16 bytes, two accesses for eight of fp32 - and as fp32 values.
+template <unsigned E> struct Few {
+  float f[E];
 };
-template <int TY>
-__device__ __forceinline__ Raw<TY> clip_load8(const void* p, unsigned g) {
-  Raw<TY> r{};
-  if constexpr (TY == TY_F32) {
-    r.a = *dev<u32x4_a4>(p, g * 32u);
-    r.b = *dev<u32x4_a4>(p, g * 32u + 16u);
-  } else {
-    r.a = *dev<u32x4_a2>(p, g * 16u);
-  }
-  return r;
-}
-template <int TY>
-__device__ __forceinline__ f32x8 clip_widen(const Raw<TY>& r) {
-  f32x8 v;
-  if constexpr (TY == TY_F32) {
+template <int TY, unsigned E> struct FewRaw {
+  static constexpr unsigned WORDS = TY == TY_F32 ? E : E / 2;
+  unsigned w[WORDS];
+  __device__ __forceinline__ void load(const void* p, unsigned g) {
+    if constexpr (WORDS == 2) {
+      const u32x2 v = *dev<u32x2_a2>(p, g * 8u);
+      w[0] = v[0];
+      w[1] = v[1];
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = __uint_as_float(r.a[i]);
-      v[4 + i] = __uint_as_float(r.b[i]);
+      for (unsigned q = 0; q < WORDS / 4; ++q) {
+        const u32x4 v = *dev<u32x4_a2>(p, g * (WORDS * 4u) + q * 16u);
+#pragma unroll
+        for (unsigned i = 0; i < 4; ++i) w[q * 4 + i] = v[i];
+      }
     }
-  } else if constexpr (TY == TY_BF16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(r.a[i] << 16);
-      v[2 * i + 1] = __uint_as_float(r.a[i] & 0xffff0000u);
-    }
-  } else {
-    const f16x8 h = __builtin_bit_cast(f16x8, r.a);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
   }
-  return v;
-}
+  __device__ __forceinline__ Few<E> widen() const {
+    Few<E> r;
+#pragma unroll
+    for (unsigned i = 0; i < E; ++i) {
+      if constexpr (TY == TY_F32) r.f[i] = __uint_as_float(w[i]);
+      else if constexpr (TY == TY_BF16) r.f[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      else r.f[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+    }
+    return r;
+  }
+};
 // rounded to nearest even; NT: not kept in the caches
 template <typename V, bool NT, typename U>
 __device__ __forceinline__ void clip_put(void* p, unsigned byte, U v) {
   if (NT) __builtin_nontemporal_store((V)v, dev<V>(p, byte));
   else *dev<V>(p, byte) = v;
 }
-template <int TY, bool NT = false>
-__device__ __forceinline__ void clip_store8(void* p, unsigned g, const f32x8& v) {
-  if constexpr (TY == TY_F32) {
-    u32x4 a, b;
+template <int TY, unsigned E, bool NT>
+__device__ __forceinline__ void few_store(void* p, unsigned g, const Few<E>& v, float k) {
+  constexpr unsigned WORDS = TY == TY_F32 ? E : E / 2;
+  unsigned w[WORDS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = __float_as_uint(v[i]);
-      b[i] = __float_as_uint(v[4 + i]);
+  for (unsigned i = 0; i < WORDS; ++i) {
+    if constexpr (TY == TY_F32) {
+      w[i] = __float_as_uint(v.f[i] * k);
+    } else {
+      typedef typename std::conditional<TY == TY_BF16, __bf16, _Float16>::type H;
+      typedef H H2 __attribute__((ext_vector_type(2)));
+      H2 h;
+      h[0] = (H)(v.f[2 * i] * k);
+      h[1] = (H)(v.f[2 * i + 1] * k);
+      w[i] = __builtin_bit_cast(unsigned, h);
     }
-    clip_put<u32x4_a4, NT>(p, g * 32u, a);
-    clip_put<u32x4_a4, NT>(p, g * 32u + 16u, b);
-  } else if constexpr (TY == TY_BF16) {
-    bf16x8 h;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = (__bf16)v[i];
-    clip_put<u32x4_a2, NT>(p, g * 16u, __builtin_bit_cast(u32x4, h));
+  }
+  if constexpr (WORDS == 2) {
+    clip_put<u32x2_a2, NT>(p, g * 8u, u32x2{w[0], w[1]});
   } else {
-    f16x8 h;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = (_Float16)v[i];
-    clip_put<u32x4_a2, NT>(p, g * 16u, __builtin_bit_cast(u32x4, h));
+    for (unsigned q = 0; q < WORDS / 4; ++q)
+      clip_put<u32x4_a2, NT>(p, g * (WORDS * 4u) + q * 16u, u32x4{w[q * 4], w[q * 4 + 1], w[q * 4 + 2], w[q * 4 + 3]});
   }
 }
 template <int TY>
@@ -141,28 +136,32 @@ struct ClipAcc {
   unsigned mx = 0;
 };
 
-// One chunk's share of thread `t` of CLIP_T.
+// One chunk's share of thread `t` of CLIP_T: 16-byte loads at consecutive addresses along the lanes, CLIP_U of them in flight.
 template <bool MAX, int TY>
 __device__ __forceinline__ void norm_chunk(const ClipChunk& ck, unsigned t, ClipAcc& acc) {
-  const unsigned groups = ck.n / CLIP_E;
-  auto add = [&](const Raw<TY>& r) {
-    const f32x8 v = clip_widen<TY>(r);
+  constexpr unsigned E = TY == TY_F32 ? 4 : 8, U = CLIP_U * CLIP_E / E;
+  const unsigned groups = ck.n / E;
+  auto add = [&](const Few<E>& v) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (MAX) acc.mx = max(acc.mx, abs_bits(v[i]));
-      else acc.sum = fma((double)v[i], (double)v[i], acc.sum);
+    for (unsigned i = 0; i < E; ++i) {
+      if (MAX) acc.mx = max(acc.mx, abs_bits(v.f[i]));
+      else acc.sum = fma((double)v.f[i], (double)v.f[i], acc.sum);
     }
   };
   unsigned g = t;
-  for (; g + (CLIP_U - 1) * CLIP_T < groups; g += CLIP_U * CLIP_T) {
-    Raw<TY> r[CLIP_U];
+  for (; g + (U - 1) * CLIP_T < groups; g += U * CLIP_T) {
+    FewRaw<TY, E> r[U];
 #pragma unroll
-    for (int u = 0; u < CLIP_U; ++u) r[u] = clip_load8<TY>(ck.src, g + u * CLIP_T);
+    for (unsigned u = 0; u < U; ++u) r[u].load(ck.src, g + u * CLIP_T);
 #pragma unroll
-    for (int u = 0; u < CLIP_U; ++u) add(r[u]);
+    for (unsigned u = 0; u < U; ++u) add(r[u].widen());
   }
-  for (; g < groups; g += CLIP_T) add(clip_load8<TY>(ck.src, g));
-  const unsigned i = groups * CLIP_E + t;
+  for (; g < groups; g += CLIP_T) {
+    FewRaw<TY, E> r;
+    r.load(ck.src, g);
+    add(r.widen());
+  }
+  const unsigned i = groups * E + t;
   if (i < ck.n) {
     const float v = clip_load1<TY>(ck.src, i);
     if (MAX) acc.mx = max(acc.mx, abs_bits(v));
@@ -177,19 +176,31 @@ __device__ __forceinline__ void norm_any(const ClipChunk& ck, unsigned t, ClipAc
   else norm_chunk<MAX, TY_F16>(ck, t, acc);
 }
 
+// Stores of a wave cover whole 128-byte lines: the elements before the destination's first line and after its last group
+// go one by one (a destination packed tight between others starts anywhere; written across lines and past the cache, 105 MB
+// became 142 MB of memory traffic).
 template <bool NT, int TS, int TD>
 __device__ __forceinline__ void scale_chunk(const ClipChunk& ck, unsigned t, float k) {
-  const unsigned groups = ck.n / CLIP_E;
+  constexpr unsigned E = TS == TY_F32 || TD == TY_F32 ? 4 : 8, U = CLIP_U * CLIP_E / E;
+  constexpr unsigned SS = TS == TY_F32 ? 4 : 2, SD = TD == TY_F32 ? 4 : 2;
+  const unsigned head = min(ck.n, (128u - ((unsigned)reinterpret_cast<uintptr_t>(ck.dst) & 127u)) % 128u / SD);
+  const unsigned groups = (ck.n - head) / E, i = head + groups * E + t;
+  const void* src = static_cast<const char*>(ck.src) + head * SS;
+  void* dst = static_cast<char*>(ck.dst) + head * SD;
+  if (t < head) clip_store1<TD>(ck.dst, t, clip_load1<TS>(ck.src, t) * k);
   unsigned g = t;
-  for (; g + (CLIP_U - 1) * CLIP_T < groups; g += CLIP_U * CLIP_T) {
-    Raw<TS> r[CLIP_U];
+  for (; g + (U - 1) * CLIP_T < groups; g += U * CLIP_T) {
+    FewRaw<TS, E> r[U];
 #pragma unroll
-    for (int u = 0; u < CLIP_U; ++u) r[u] = clip_load8<TS>(ck.src, g + u * CLIP_T);
+    for (unsigned u = 0; u < U; ++u) r[u].load(src, g + u * CLIP_T);
 #pragma unroll
-    for (int u = 0; u < CLIP_U; ++u) clip_store8<TD, NT>(ck.dst, g + u * CLIP_T, clip_widen<TS>(r[u]) * k);
+    for (unsigned u = 0; u < U; ++u) few_store<TD, E, NT>(dst, g + u * CLIP_T, r[u].widen(), k);
   }
-  for (; g < groups; g += CLIP_T) clip_store8<TD, NT>(ck.dst, g, clip_widen<TS>(clip_load8<TS>(ck.src, g)) * k);
-  const unsigned i = groups * CLIP_E + t;
+  for (; g < groups; g += CLIP_T) {
+    FewRaw<TS, E> r;
+    r.load(src, g);
+    few_store<TD, E, NT>(dst, g, r.widen(), k);
+  }
   if (i < ck.n) clip_store1<TD>(ck.dst, i, clip_load1<TS>(ck.src, i) * k);
 }
 template <bool NT, int TS>
@@ -290,35 +301,49 @@ __global__ __launch_bounds__(CLIP_SMALL_T * CLIP_SMALL_TEAMS) void norm_clip_ker
     if (team + u * CLIP_SMALL_TEAMS >= n_chunks) ck[u].n = 0;
   }
   // groups of eight, and the few elements past the last whole group; every load is issued before the first is used
-  u32x4 ra[CLIP_SMALL_U], rb[CLIP_SMALL_U];
+  FewRaw<TY_F32, 8> word[CLIP_SMALL_U];         // (16-bit types fill the first half)
   unsigned rt[CLIP_SMALL_U];
 #pragma unroll
   for (int u = 0; u < CLIP_SMALL_U; ++u) {
-    ra[u] = rb[u] = u32x4(0u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word[u].w[i] = 0u;
     rt[u] = 0u;
-    const unsigned wide = (ck[u].types & 0xff) == TY_F32 ? 1u : 0u, groups = ck[u].n / CLIP_E, i = groups * CLIP_E + t;
+    const bool wide = (ck[u].types & 0xff) == TY_F32;
+    const unsigned groups = ck[u].n / CLIP_E, i = groups * CLIP_E + t;
     if (t < groups) {
-      ra[u] = *dev<u32x4_a2>(ck[u].src, t * 16u << wide);
-      if (wide) rb[u] = *dev<u32x4_a2>(ck[u].src, t * 32u + 16u);
+      if (wide) {
+        word[u].load(ck[u].src, t);
+      } else {
+        FewRaw<TY_BF16, 8> h;
+        h.load(ck[u].src, t);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) word[u].w[q] = h.w[q];
+      }
     }
     if (i < ck[u].n) {
       if (wide) rt[u] = *dev<unsigned>(ck[u].src, i * 4u);
       else rt[u] = *dev<uint16_t>(ck[u].src, i * 2u);
     }
   }
-  f32x8 v[CLIP_SMALL_U];
+  Few<8> v[CLIP_SMALL_U];
   float tail[CLIP_SMALL_U];
 #pragma unroll
   for (int u = 0; u < CLIP_SMALL_U; ++u) {
     const unsigned ty = ck[u].types & 0xff;
     if (ty == TY_F32) {
-      v[u] = clip_widen<TY_F32>(Raw<TY_F32>{ra[u], rb[u]});
+      v[u] = word[u].widen();
       tail[u] = __uint_as_float(rt[u]);
     } else if (ty == TY_BF16) {
-      v[u] = clip_widen<TY_BF16>(Raw<TY_BF16>{ra[u], rb[u]});
+      FewRaw<TY_BF16, 8> h;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h.w[q] = word[u].w[q];
+      v[u] = h.widen();
       tail[u] = __uint_as_float(rt[u] << 16);
     } else {
-      v[u] = clip_widen<TY_F16>(Raw<TY_F16>{ra[u], rb[u]});
+      FewRaw<TY_F16, 8> h;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h.w[q] = word[u].w[q];
+      v[u] = h.widen();
       tail[u] = (float)__builtin_bit_cast(_Float16, (uint16_t)rt[u]);
     }
   }
@@ -327,8 +352,8 @@ __global__ __launch_bounds__(CLIP_SMALL_T * CLIP_SMALL_TEAMS) void norm_clip_ker
   for (int u = 0; u < CLIP_SMALL_U; ++u) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (MAX) acc.mx = max(acc.mx, abs_bits(v[u][i]));
-      else acc.sum = fma((double)v[u][i], (double)v[u][i], acc.sum);
+      if (MAX) acc.mx = max(acc.mx, abs_bits(v[u].f[i]));
+      else acc.sum = fma((double)v[u].f[i], (double)v[u].f[i], acc.sum);
     }
     if (MAX) acc.mx = max(acc.mx, abs_bits(tail[u]));
     else acc.sum = fma((double)tail[u], (double)tail[u], acc.sum);
@@ -341,9 +366,9 @@ __global__ __launch_bounds__(CLIP_SMALL_T * CLIP_SMALL_TEAMS) void norm_clip_ker
   for (int u = 0; u < CLIP_SMALL_U; ++u) {
     const unsigned td = ck[u].types >> 8, groups = ck[u].n / CLIP_E, i = groups * CLIP_E + t;
     if (t < groups) {
-      if (td == TY_F32) clip_store8<TY_F32>(ck[u].dst, t, v[u] * k);
-      else if (td == TY_BF16) clip_store8<TY_BF16>(ck[u].dst, t, v[u] * k);
-      else clip_store8<TY_F16>(ck[u].dst, t, v[u] * k);
+      if (td == TY_F32) few_store<TY_F32, 8, false>(ck[u].dst, t, v[u], k);
+      else if (td == TY_BF16) few_store<TY_BF16, 8, false>(ck[u].dst, t, v[u], k);
+      else few_store<TY_F16, 8, false>(ck[u].dst, t, v[u], k);
     }
     if (i < ck[u].n) {
       if (td == TY_F32) clip_store1<TY_F32>(ck[u].dst, i, tail[u] * k);
