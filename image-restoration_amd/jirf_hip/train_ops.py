@@ -168,10 +168,13 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
     L = lib()
     dense = like.is_contiguous()
     dx, df = _new(like, dense) if k1 else dy, _new(like, dense)
-    # the [C] gradients are rows of one tensor
+    # the [C] gradients: rows of one tensor where there are several
     rows = [None] * 5
     wanted = [i for i, on in enumerate((k0, b0 is not None, gk == 1, k1, b1 is not None)) if on]
-    if wanted:
+    if len(wanted) < 3:
+        for i in wanted:
+            rows[i] = like.new_empty(Cn, dtype=torch.float32)
+    else:
         for i, t in zip(wanted, like.new_empty((len(wanted), Cn), dtype=torch.float32).unbind()):
             rows[i] = t
     if gk == 2:
