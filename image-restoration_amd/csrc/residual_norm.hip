@@ -111,7 +111,12 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
   if ((f.tok ? a.C : a.P) < vec || image_bytes >= 1l << 32) {
     f.lanes = -1;
   } else if (f.tok) {
-    // eight channels per thread; sixteen where eight would need more than 512 threads
+    // Eight channels per thread, in groups of lanes that share a wave up to 512 channels (22 channels: groups of four lanes
+    // against eight, backward of 524288 tokens fp32 67 / 73 us, bf16 52 / 71 us).  Sixteen where eight would need more than
+    // 512 threads; in the backward of 16-bit types from 2049 channels on, half as many waves (2x6464x2163 fp16 113 us
+    // against 126 with eight, 4x1066x3344 29 / 32).  Not where that loses: fp32 (2x3464x2600 88 / 84 us), no norm and no gate
+    // on the branch (8x1066x4096 bf16 73 / 65), a gate per image, whose sums close with every image: short images lose more
+    // (16x300x4096 bf16 82 / 70, 64x37x2300 71 / 67) than long ones gain (2x6464x2600 fp16 125 / 129).
     const int threads8 = (a.C + 7) / 8;
     const bool wide16 = backward && dtype != JIRF_F32 && a.gate_kind != 2 && (a.post || a.gate_kind);
     f.nv = 8 / vec;
@@ -129,7 +134,9 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
     }
   } else {
     // four channels of four pixels per thread: as many pixel lanes (of 32) as the channels leave room for in 256 threads,
-    // more threads only to keep eight lanes (a 128-byte line of fp32), or fewer lanes than that to fit at all
+    // more threads only to keep eight lanes (a 128-byte line of fp32: backward of 4x256x16384 with 512 threads 109 us, with
+    // four lanes in 256 threads 131 us), or fewer lanes than that to fit at all.  The 16-bit forward has registers for 1024
+    // threads (3x567x49959 bf16 272 us; with 512 at most 382 us).
     const int rows = (a.C + 3) / 4, most = !backward && dtype != JIRF_F32 ? 1024 : 512;
     f.nv = 4;
     f.lanes = 32;
