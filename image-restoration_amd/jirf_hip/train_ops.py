@@ -47,9 +47,10 @@ def _sizes(x: torch.Tensor, layout: str):
         raise ValueError(f"{layout} activations are [B, C, ...] / [B, P, C], got shape {tuple(shape)}")
     if n == 0:
         raise ValueError(f"empty activation {tuple(shape)}")
-    if lay:
-        return shape[0], shape[2], shape[1], lay, dtype
-    return shape[0], shape[1], n // (shape[0] * shape[1]), lay, dtype
+    B, Cn, P = (shape[0], shape[2], shape[1]) if lay else (shape[0], shape[1], n // (shape[0] * shape[1]))
+    if n >> 31 and (B >> 31 or Cn >> 31 or P >> 31):        # a C int would keep the low bits
+        raise ValueError(f"{layout} activation {tuple(shape)}: images, channels and pixels have to fit 31 bits each")
+    return B, Cn, P, lay, dtype
 
 
 def _bs(name: str, t: torch.Tensor, like: torch.Tensor) -> int:

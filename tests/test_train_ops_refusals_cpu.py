@@ -139,3 +139,25 @@ def test_python_layer_refuses_parameters():
     for gate in (torch.zeros(6), torch.zeros(2, 8), torch.zeros(3, 8, 6), good.bfloat16()):
         with pytest.raises(ValueError):
             T._gate(gate, 3, 8, like)
+
+
+@pytest.mark.parametrize("layout,shape", [("planar", (1, 1, 2**16, 2**16 + 5)), ("planar", (1, 1, 2**31)), ("tokens", (1, 2**32 + 5, 1)),
+                                          ("planar", (2**32 + 5, 1, 1)), ("tokens", (1, 1, 2**31))])
+def test_sizes_past_31_bits_are_refused_not_cut_off(layout, shape):
+    x = torch.empty(shape, dtype=torch.float16, device="meta")
+
+    class OnGpu:
+        is_cuda, dtype, numel = True, x.dtype, x.numel
+    OnGpu.shape = x.shape
+    with pytest.raises(ValueError, match="31 bits"):
+        T._sizes(OnGpu, layout)
+
+
+def test_the_largest_size_of_31_bits_is_taken():
+    class OnGpu:
+        is_cuda, dtype, shape = True, torch.float16, torch.Size((1, 2, 2**31 - 1))
+
+        @staticmethod
+        def numel():
+            return 2 * (2**31 - 1)
+    assert T._sizes(OnGpu, "planar")[:3] == (1, 2, 2**31 - 1)
