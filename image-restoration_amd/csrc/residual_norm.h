@@ -331,6 +331,8 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
   typedef Tile<T, TOK, L, NV, VEC, NT> Ti;
   typedef typename Ti::Vec Vec;
   constexpr int NS = Ti::NS, NP = Ti::NP;
+  // the next tile is fetched ahead where the registers (256 per thread) have room for two tiles
+  constexpr bool PF = NV * VEC * sizeof(T) < 128;
   __shared__ __attribute__((aligned(32))) float lds[Ti::RED];
   Ti ti(a, lds);
   int b0, b1, t0;
@@ -339,8 +341,10 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
   if (b0 >= b1 || t0 >= t1) return;           // (uniform over the threads of a worker, and a worker's barriers are its own)
   float pw[NV][NP], pb[NV][NP], gw[NV][NP], gb[NV][NP];
   Vec xn[NV], fn[NV];
-  ti.load(Ti::image(a.f, a.f_bs, b0), ti.start(t0), fn);
-  ti.load(Ti::image(a.x, a.x_bs, b0), ti.start(t0), xn);
+  if (PF) {
+    ti.load(Ti::image(a.f, a.f_bs, b0), ti.start(t0), fn);
+    ti.load(Ti::image(a.x, a.x_bs, b0), ti.start(t0), xn);
+  }
   ti.params(a.pre ? a.pre_w : nullptr, 0.f, pw);
   ti.params(a.pre == 1 ? a.pre_b : nullptr, 0.f, pb);
   int gate_of = -1;
@@ -363,6 +367,10 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
     }
     const float s = a.scale ? a.scale[b] : 1.0f;
     for (int t = t0; t < t1; t += a.S) {
+      if (!PF) {
+        ti.load(Ti::image(a.f, a.f_bs, b), ti.start(t), fn);
+        ti.load(Ti::image(a.x, a.x_bs, b), ti.start(t), xn);
+      }
       Vec xv[NV], fv[NV];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -370,7 +378,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
         fv[j] = fn[j];
       }
       const int bn = t + a.S < t1 ? b : b + 1, tn = t + a.S < t1 ? t + a.S : t0;
-      if (bn < b1) {
+      if (PF && bn < b1) {
         ti.load(Ti::image(a.f, a.f_bs, bn), ti.start(tn), fn);
         ti.load(Ti::image(a.x, a.x_bs, bn), ti.start(tn), xn);
       }
@@ -992,8 +1000,20 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
         }
     }
   } else {
+    if constexpr (sizeof(T) == 4) {
+      if (f.nv == 8) {
+        switch (f.lanes) {
+          case 2: RN_FWD(false, 2, 8); break;
+          case 4: RN_FWD(false, 4, 8); break;
+          default: RN_FWD(false, 8, 8);
+        }
+        return;
+      }
+    }
     switch (f.lanes) {
-      case 2: RN_FWD(false, 2, 4); break;
+      case 2:
+        if constexpr (sizeof(T) == 2) RN_FWD(false, 2, 4);
+        break;
       case 4: RN_FWD(false, 4, 4); break;
       case 8: RN_FWD(false, 8, 4); break;
       case 16: RN_FWD(false, 16, 4); break;

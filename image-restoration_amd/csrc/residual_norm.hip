@@ -137,8 +137,16 @@ RnForm choose_form(RnArgs& a, int dtype, int layout, bool backward) {
     // more threads only to keep eight lanes (a 128-byte line of fp32: backward of 4x256x16384 with 512 threads 109 us, with
     // four lanes in 256 threads 131 us), or fewer lanes than that to fit at all.  The 16-bit forward has registers for 1024
     // threads (3x567x49959 bf16 272 us; with 512 at most 382 us).
-    const int rows = (a.C + 3) / 4, most = !backward && dtype != JIRF_F32 ? 1024 : 512;
-    f.nv = 4;
+    // Eight channels of four pixels in the fp32 forward where eight lanes of four would need more than 256 threads, which keeps
+    // eight lanes up to 512 channels and four up to 1024: 4x512x16384 182 -> 133 us, 4x300x16384 91 -> 68, 4x256x16384
+    // 57 -> 50, 4x700x16384 251 -> 232; 4x128x16384 would lose (25.7 -> 26.2).  Not below 256 tiles while four channels keep
+    // four lanes (8x140x300 5.1 -> 6.7).  The backward and the 16-bit forward gain at some sizes and lose at others
+    // (backward without a branch norm 4x300x16384 104 -> 100, 12x256x4096 50 -> 61; with one it spills some 190 registers;
+    // bf16 4x256x16384 39 -> 35, 4x200x16384 27 -> 29).
+    const int most = !backward && dtype != JIRF_F32 ? 1024 : 512;
+    const bool eight = !backward && dtype == JIRF_F32 && a.C > 128 && (a.C > 512 || ((long)a.P + 31) / 32 * a.B >= 256);
+    f.nv = eight ? 8 : 4;
+    const int rows = (a.C + f.nv - 1) / f.nv;
     f.lanes = 32;
     while (f.lanes > 8 && f.lanes * rows > 256) f.lanes >>= 1;
     while (f.lanes > 2 && f.lanes * rows > most) f.lanes >>= 1;

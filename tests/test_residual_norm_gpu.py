@@ -483,3 +483,27 @@ def test_calls_larger_than_the_cache(dtype, C, P):
     # at most P / 256 rows in 32 bits
     for k, v in sums.items():
         assert (gb[k].double() - v).abs().max() <= (P / 256 + 60) * 2.0 ** -24 * 8 * P, k
+
+
+# fp32 planes of more than 128 channels, forward: eight, four and two pixel lanes; ragged channels and pixels; the last two
+# with more tiles than workers
+@pytest.mark.parametrize("B,C,P", [(9, 131, 1003), (64, 300, 130), (4, 511, 2055), (300, 257, 5), (2, 700, 50), (1, 1024, 9),
+                                   (3, 1025, 21), (1, 2047, 401), (1, 2048, 4), (8, 512, 2055), (33, 131, 2011)])
+def test_planes_of_many_channels(B, C, P):
+    for i, (post, gate, pre, scale) in enumerate([(1, 2, 1, True), (3, 1, 2, False), (0, 0, 3, True)][:1 if B * C * P > 5e6 else 3]):
+        d = make("planar", F32, B, C, P, post, gate, pre, scale, seed=30 + i)
+        r = run_both(d, "planar", R.chain(C, "planar"), backward=False)
+        kw = dict(post=d["post"], gate=d["gate"], scale=d["scale"], pre=d["pre"])
+        x, f = d["x"].clone(), d["f"].clone()
+        T.residual_norm(x, f, out=x, norm_out=f, **kw)
+        assert torch.equal(x, r.y) and torch.equal(f, r.n)
+        # a pixel of infinities is nobody else's: every other pixel keeps its bits
+        for back in (1, 3, 4, 5):
+            if back > P:
+                continue
+            x = d["x"].clone()
+            x[:, :, P - back] = float("inf")
+            s = T.residual_norm(x, d["f"], **kw)
+            others = torch.arange(P, device="cuda") != P - back
+            assert torch.equal(s.y[..., others], r.y[..., others]) and torch.equal(s.n[..., others], r.n[..., others])
+            assert torch.isinf(s.y[..., P - back]).all()
