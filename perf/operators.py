@@ -163,19 +163,13 @@ def prepare(case, seed):
     return st
 
 
-_train_ops = None
-
-
 def _ops():
-    """The framework's operators on torch tensors, imported once as a program does."""
-    global _train_ops
-    if _train_ops is None:
-        pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "image-restoration_amd")
-        if pkg not in sys.path:
-            sys.path.insert(0, pkg)
-        from jirf_hip import train_ops
-        _train_ops = train_ops
-    return _train_ops
+    """The framework's operators on torch tensors."""
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "image-restoration_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from jirf_hip import train_ops
+    return train_ops
 
 
 def run(st):
