@@ -19,6 +19,7 @@
 // not from the rounded y, and the statistics saved for the backward are those of the fp32 values.  Parameters, gate, scale,
 // statistics and parameter gradients are fp32.  No atomics: every sum has a fixed order.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "residual_norm.h"
@@ -44,6 +45,8 @@ int guarded_r(F&& f) {
 
 bool kind_ok(int k) { return k >= 0 && k <= 3; }
 bool dtype_ok(int d) { return d == JIRF_F32 || d == JIRF_BF16 || d == JIRF_F16; }
+// Channel indices are 32 bits and step up to 256 past the last channel.
+constexpr int RN_MOST_C = INT_MAX - 511;
 
 void check_common(const char* who, int dtype, int layout, int post, const float* post_w, int gate_kind, const float* gate, int pre,
                   const float* pre_w, int B, int C, int P) {
@@ -54,6 +57,7 @@ void check_common(const char* who, int dtype, int layout, int post, const float*
   JIRF_REQUIRE((!post || post_w) && (!pre || pre_w) && (!gate_kind || gate), JIRF_EINVAL,
                "%s: a norm without its weight or a gate without its factors", who);
   JIRF_REQUIRE(B > 0 && C > 0 && P > 0, JIRF_EINVAL, "%s: sizes B %d C %d P %d", who, B, C, P);
+  JIRF_REQUIRE(C <= RN_MOST_C, JIRF_EINVAL, "%s: %d channels, at most %d", who, C, RN_MOST_C);
 }
 // Batch stride of one tensor (0: dense).  An image's C * P elements are contiguous; images of an output may not overlap.
 long batch_stride(const char* who, const char* name, const void* p, long bs, int dtype, int B, int C, int P) {
@@ -340,7 +344,7 @@ int jirf_train_residual_norm(const void* x, long x_bs, const void* f, long f_bs,
 
 long jirf_train_residual_norm_bwd_work_floats(int dtype, int layout, int post_kind, int gate_kind, int pre_kind, int B, int C, int P) {
   if (!dtype_ok(dtype) || (layout != JIRF_LAYOUT_PLANAR && layout != JIRF_LAYOUT_TOKENS) || !kind_ok(post_kind) ||
-      !kind_ok(pre_kind) || gate_kind < 0 || gate_kind > 2 || B <= 0 || C <= 0 || P <= 0)
+      !kind_ok(pre_kind) || gate_kind < 0 || gate_kind > 2 || B <= 0 || C <= 0 || C > RN_MOST_C || P <= 0)
     return -1;
   RnArgs a{};
   a.post = post_kind; a.pre = pre_kind; a.gate_kind = gate_kind; a.B = B; a.C = C; a.P = P;

@@ -452,7 +452,8 @@ int jirf_train_window_attention_bwd(const float* qkv, long qkv_bs, const float* 
  *   gate_kind  0 none, 1 gate [C], 2 gate [B][C];   scale [B] or NULL
  *   stats      NULL, or [4][B][P] for the backward: mean and reciprocal deviation of f, then of y (0 where there is no
  *              norm; mean 0 for kind 3)
- * Parameters, gate, scale and stats are fp32.  y may be x and n may be f; other outputs overlap nothing. */
+ * Parameters, gate, scale and stats are fp32.  y may be x and n may be f; other outputs overlap nothing.  At most 2^31 - 512
+ * channels. */
 #define JIRF_LAYOUT_PLANAR 0
 #define JIRF_LAYOUT_TOKENS 1
 int jirf_train_residual_norm(const void* x, long x_bs, const void* f, long f_bs, int dtype, int layout, int post_kind,

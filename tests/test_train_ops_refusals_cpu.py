@@ -161,3 +161,21 @@ def test_the_largest_size_of_31_bits_is_taken():
         def numel():
             return 2 * (2**31 - 1)
     assert T._sizes(OnGpu, "planar")[:3] == (1, 2, 2**31 - 1)
+
+
+MOST_C = 2**31 - 512       # channel indices step by up to 256 past the last channel in 32 bits
+
+
+@pytest.mark.parametrize("dtype,layout", [(4, 1), (5, 1), (0, 1), (4, 0), (0, 0)])
+def test_more_channels_than_an_index_holds_are_refused(dtype, layout):
+    """Where (C + 7) / 8 no longer fits 32 bits, a kernel for 32 channels would be chosen; refused from 256 steps before."""
+    size = jirf_hip.lib().jirf_train_residual_norm_bwd_work_floats
+    for C_ in (MOST_C + 1, 2**31 - 8, 2**31 - 7, 2**31 - 1):
+        assert fwd(dtype=dtype, layout=layout, B=1, C=C_, P=1, f=D, y=0x100_0000_0000) == EINVAL, C_
+        assert "channels" in jirf_hip.last_error()
+        assert bwd(dtype=dtype, layout=layout, B=1, C=C_, P=1, dx=None, df=0x100_0000_0000) == EINVAL, C_
+        assert "channels" in jirf_hip.last_error()
+        assert size(dtype, layout, 0, 0, 1, 1, C_, 1) < 0, C_
+    # the kernel for any number of channels up to there: two row sums per pixel, four rows of partial sums
+    for C_ in (16384 + 1, 2**28, 2**30 + 3, MOST_C):
+        assert size(dtype, layout, 0, 0, 1, 1, C_, 1) == 2 + 4 * C_, C_
