@@ -47,6 +47,9 @@ bool kind_ok(int k) { return k >= 0 && k <= 3; }
 bool dtype_ok(int d) { return d == JIRF_F32 || d == JIRF_BF16 || d == JIRF_F16; }
 // Channel indices are 32 bits and step up to 256 past the last channel.
 constexpr int RN_MOST_C = INT_MAX - 511;
+// The launches that sum the parameter gradients have up to 64 threads per channel (RED_C columns of RED_R rows; planar, four
+// channels of 256 threads), and a grid holds fewer than 2^32 threads.
+constexpr int RN_MOST_C_PARAMS = (1 << 26) - 16;
 
 void check_common(const char* who, int dtype, int layout, int post, const float* post_w, int gate_kind, const float* gate, int pre,
                   const float* pre_w, int B, int C, int P) {
@@ -368,7 +371,9 @@ int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, lon
     JIRF_REQUIRE((!dpost_w || post_kind) && (!dpost_b || post_kind == 1) && (!dgate || gate_kind) && (!dpre_w || pre_kind) &&
                      (!dpre_b || pre_kind == 1),
                  JIRF_EINVAL, "%s: a parameter gradient without its norm or gate", who);
-    JIRF_REQUIRE(!(dpost_w || dpost_b || dgate || dpre_w || dpre_b || pre_kind) || work, JIRF_EINVAL, "%s: null work", who);
+    const bool params = dpost_w || dpost_b || dgate || dpre_w || dpre_b;
+    JIRF_REQUIRE(!(params || pre_kind) || work, JIRF_EINVAL, "%s: null work", who);
+    JIRF_REQUIRE(!params || C <= RN_MOST_C_PARAMS, JIRF_EINVAL, "%s: parameter gradients of %d channels, at most %d", who, C, RN_MOST_C_PARAMS);
     RnArgs a{};
     a.dy = dy; a.dn = dn; a.y_in = y; a.f = f; a.dx = dx; a.df = df;
     a.dy_bs = batch_stride(who, "dy", dy, dy_bs, dtype, B, C, P);
@@ -392,7 +397,6 @@ int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, lon
     const RnForm form = choose_form(a, dtype, layout, true);
     const BwdWork wk = bwd_work(a, form);
     const bool branch = post_kind || gate_kind;
-    const bool params = dpost_w || dpost_b || dgate || dpre_w || dpre_b;
     if (work) {
       a.rowsum = work;
       a.part = params ? work + wk.rowsum : nullptr;

@@ -464,10 +464,10 @@ int jirf_train_residual_norm(const void* x, long x_bs, const void* f, long f_bs,
  * forward's, f its branch input (NULL where neither norm nor gate sits on the branch; dn, y NULL without N_pre).
  *     dx = dy + dN_pre(dn),   df = dN_post(scale * gate * dx)     (without N_pre dx is dy: it may be NULL, not written)
  * and the parameter gradients dpost_w, dpost_b, dpre_w, dpre_b [C], dgate [C] or [B][C], each NULL when not wanted,
- * accumulate != 0 adds to them.  No gradient for scale (it is drawn, not learned).  work: DEVICE memory of
- * jirf_train_residual_norm_bwd_work_floats() floats owned by the caller, needed only during the call (calls that
- * run at the same time need one each); that function returns < 0 for bad arguments.  Outputs overlap nothing.
- * Sums have a fixed order (no atomics). */
+ * accumulate != 0 adds to them; at most 2^26 - 16 channels where one is wanted.  No gradient for scale (it is drawn,
+ * not learned).  work: DEVICE memory of jirf_train_residual_norm_bwd_work_floats() floats owned by the caller, needed
+ * only during the call (calls that run at the same time need one each); that function returns < 0 for bad arguments.
+ * Outputs overlap nothing.  Sums have a fixed order (no atomics). */
 long jirf_train_residual_norm_bwd_work_floats(int dtype, int layout, int post_kind, int gate_kind, int pre_kind, int B, int C,
                                               int P);
 int jirf_train_residual_norm_bwd(const void* dy, long dy_bs, const void* dn, long dn_bs, const void* y, long y_bs, const void* f,

@@ -179,3 +179,18 @@ def test_more_channels_than_an_index_holds_are_refused(dtype, layout):
     # the kernel for any number of channels up to there: two row sums per pixel, four rows of partial sums
     for C_ in (16384 + 1, 2**28, 2**30 + 3, MOST_C):
         assert size(dtype, layout, 0, 0, 1, 1, C_, 1) == 2 + 4 * C_, C_
+
+
+@pytest.mark.parametrize("layout", [0, 1])
+def test_parameter_gradients_of_more_channels_than_a_grid_holds_are_refused(layout):
+    """The sums over the rows take 64 threads per channel in one grid of fewer than 2^32 threads; without parameter gradients
+    there is no such launch."""
+    far = 0x100_0000_0000
+    for C_ in (2**26 - 15, 2**26, MOST_C):
+        kw = dict(layout=layout, pre=2, pre_w=A, dy=None, dn=A, y=B_, stats=D, work=D, dx=far, df=2 * far, dpre_w=E, B=1, C=C_, P=1)
+        assert bwd(**kw) == EINVAL and "parameter gradients" in jirf_hip.last_error(), C_
+        assert bwd(**dict(kw, pre=0, gate_kind=1, gate=A, f=A, dy=A, dn=None, dx=None, dpre_w=None, dgate=E)) == EINVAL
+        assert "parameter gradients" in jirf_hip.last_error(), C_
+    if not torch.cuda.is_available():        # nothing to launch on: the arguments themselves are taken
+        assert bwd(**dict(kw, dpre_w=None)) != EINVAL
+        assert bwd(**dict(kw, C=2**26 - 16)) != EINVAL
