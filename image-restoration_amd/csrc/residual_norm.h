@@ -893,7 +893,7 @@ __global__ __launch_bounds__(256) void rn_bwd_params_sweep(const RnArgs a) {
   __shared__ float red[256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int worker = blockIdx.y;
-  const int b0 = a.S > 1 ? worker / a.S : worker * a.ipw, b1 = min(a.B, a.S > 1 ? b0 + 1 : b0 + a.ipw);
+  const int b0 = a.S > 1 ? worker / a.S : worker * a.ipw, b1 = (int)min((long)a.B, (long)b0 + a.ipw);   // (S > 1: ipw is 1)
   const int slab = a.S > 1 ? worker % a.S : 0;
   const long per = ((long)a.P + a.S - 1) / a.S, p0 = min((long)a.P, slab * per), p1 = min((long)a.P, p0 + per);
   const long bp = (long)a.B * a.P;
