@@ -90,26 +90,44 @@ template <int TY, unsigned E> struct FewRaw {
     return r;
   }
 };
+// A factor outside the normal range of 32 bits (a norm of 1e38 with max_norm 0.01, a grad_scale of 1e60): a factor of order
+// one and a power of two on the side where the product stays in range.  (Multiplying in 64 bits instead takes 100 registers
+// for 38 in clip_kernel, and spills 241 in norm_clip_kernel.)
+struct FarFactor {
+  float m;
+  int before, after;      // exponents; one of them is 0
+};
+__device__ __forceinline__ FarFactor far_factor(double k) {
+  int e;
+  const double f = frexp(k, &e);                                      // [1/2, 1)
+  return k < 1.0 ? FarFactor{(float)f, 0, e} : FarFactor{(float)(2.0 * f), e - 1, 0};
+}
+__device__ __forceinline__ float scaled(float g, float k) { return g * k; }
+__device__ __forceinline__ float scaled(float g, const FarFactor& k) {
+  return __builtin_amdgcn_ldexpf(__builtin_amdgcn_ldexpf(g, k.before) * k.m, k.after);
+}
+__device__ __forceinline__ bool is_one(float k) { return k == 1.0f; }
+__device__ __forceinline__ bool is_one(const FarFactor&) { return false; }
 // rounded to nearest even; NT: not kept in the caches
 template <typename V, bool NT, typename U>
 __device__ __forceinline__ void clip_put(void* p, unsigned byte, U v) {
   if (NT) __builtin_nontemporal_store((V)v, dev<V>(p, byte));
   else *dev<V>(p, byte) = v;
 }
-template <int TY, unsigned E, bool NT>
-__device__ __forceinline__ void few_store(void* p, unsigned g, const Few<E>& v, float k) {
+template <int TY, unsigned E, bool NT, typename K>
+__device__ __forceinline__ void few_store(void* p, unsigned g, const Few<E>& v, K k) {
   constexpr unsigned WORDS = TY == TY_F32 ? E : E / 2;
   unsigned w[WORDS];
 #pragma unroll
   for (unsigned i = 0; i < WORDS; ++i) {
     if constexpr (TY == TY_F32) {
-      w[i] = __float_as_uint(v.f[i] * k);
+      w[i] = __float_as_uint(scaled(v.f[i], k));
     } else {
       typedef typename std::conditional<TY == TY_BF16, __bf16, _Float16>::type H;
       typedef H H2 __attribute__((ext_vector_type(2)));
       H2 h;
-      h[0] = (H)(v.f[2 * i] * k);
-      h[1] = (H)(v.f[2 * i + 1] * k);
+      h[0] = (H)scaled(v.f[2 * i], k);
+      h[1] = (H)scaled(v.f[2 * i + 1], k);
       w[i] = __builtin_bit_cast(unsigned, h);
     }
   }
@@ -184,15 +202,15 @@ __device__ __forceinline__ void norm_any(const ClipChunk& ck, unsigned t, ClipAc
 // Stores of a wave cover whole 128-byte lines: the elements before the destination's first line and after its last group
 // go one by one (a destination packed tight between others starts anywhere; written across lines and past the cache, 105 MB
 // became 142 MB of memory traffic).
-template <bool NT, int TS, int TD>
-__device__ __forceinline__ void scale_chunk(const ClipChunk& ck, unsigned t, float k) {
+template <bool NT, int TS, int TD, typename K>
+__device__ __forceinline__ void scale_chunk(const ClipChunk& ck, unsigned t, K k) {
   constexpr unsigned E = TS == TY_F32 || TD == TY_F32 ? 4 : 8, U = CLIP_U * CLIP_E / E;
   constexpr unsigned SS = TS == TY_F32 ? 4 : 2, SD = TD == TY_F32 ? 4 : 2;
   const unsigned head = min(ck.n, (128u - ((unsigned)reinterpret_cast<uintptr_t>(ck.dst) & 127u)) % 128u / SD);
   const unsigned groups = (ck.n - head) / E, i = head + groups * E + t;
   const void* src = static_cast<const char*>(ck.src) + head * SS;
   void* dst = static_cast<char*>(ck.dst) + head * SD;
-  if (t < head) clip_store1<TD>(ck.dst, t, clip_load1<TS>(ck.src, t) * k);
+  if (t < head) clip_store1<TD>(ck.dst, t, scaled(clip_load1<TS>(ck.src, t), k));
   unsigned g = t;
   for (; g + (U - 1) * CLIP_T < groups; g += U * CLIP_T) {
     FewRaw<TS, E> r[U];
@@ -206,20 +224,20 @@ __device__ __forceinline__ void scale_chunk(const ClipChunk& ck, unsigned t, flo
     r.load(src, g);
     few_store<TD, E, NT>(dst, g, r.widen(), k);
   }
-  if (i < ck.n) clip_store1<TD>(ck.dst, i, clip_load1<TS>(ck.src, i) * k);
+  if (i < ck.n) clip_store1<TD>(ck.dst, i, scaled(clip_load1<TS>(ck.src, i), k));
 }
-template <bool NT, int TS>
-__device__ __forceinline__ void scale_to(const ClipChunk& ck, unsigned t, float k) {
+template <bool NT, int TS, typename K>
+__device__ __forceinline__ void scale_to(const ClipChunk& ck, unsigned t, K k) {
   const unsigned td = ck.types >> 8;
   if (td == TY_F32) scale_chunk<NT, TS, TY_F32>(ck, t, k);
   else if (td == TY_BF16) scale_chunk<NT, TS, TY_BF16>(ck, t, k);
   else scale_chunk<NT, TS, TY_F16>(ck, t, k);
 }
-template <bool NT>
-__device__ __forceinline__ void scale_any(const ClipChunk& ck, unsigned t, float k) {
+template <bool NT, typename K>
+__device__ __forceinline__ void scale_any(const ClipChunk& ck, unsigned t, K k) {
   const unsigned ts = ck.types & 0xff;
   // in place with factor 1 every value stays as it is
-  if (k == 1.0f && ck.src == ck.dst && ts == ck.types >> 8) return;
+  if (is_one(k) && ck.src == ck.dst && ts == ck.types >> 8) return;
   if (ts == TY_F32) scale_to<NT, TY_F32>(ck, t, k);
   else if (ts == TY_BF16) scale_to<NT, TY_BF16>(ck, t, k);
   else scale_to<NT, TY_F16>(ck, t, k);
@@ -244,7 +262,7 @@ __device__ __forceinline__ double block_combine(double v, double* red) {
 }
 
 template <bool MAX>
-__device__ __forceinline__ float clip_factor(double raw, double max_norm, double grad_scale, double* stats, bool write) {
+__device__ __forceinline__ double clip_factor(double raw, double max_norm, double grad_scale, double* stats, bool write) {
   const double total = grad_scale * (MAX ? raw : sqrt(raw));
   double k = grad_scale;
   if (max_norm > 0.0) {
@@ -256,8 +274,10 @@ __device__ __forceinline__ float clip_factor(double raw, double max_norm, double
     stats[1] = total;
     stats[2] = k;
   }
-  return (float)k;
+  return k;
 }
+// Whether 32 bits hold the factor to 24 digits (0 and NaN as they are).
+__device__ __forceinline__ bool fits32(double k) { return k == 0.0 || k != k || (k >= 0x1p-126 && k < 0x1p127); }
 
 template <bool MAX>
 __global__ __launch_bounds__(CLIP_T) void norm_kernel(const ClipChunk* __restrict__ chunks, int n_chunks,
@@ -283,8 +303,13 @@ __global__ __launch_bounds__(CLIP_T) void clip_kernel(const ClipChunk* __restric
   double t = 0.0;
   for (int i = threadIdx.x; i < n_part; i += CLIP_T) t = combine2<MAX>(t, part[i]);
   const double raw = block_combine<MAX, CLIP_T>(t, red);
-  const float k = clip_factor<MAX>(raw, max_norm, grad_scale, stats, blockIdx.x == 0 && threadIdx.x == 0);
-  for (int c = n_chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) scale_any<NT>(chunks[c], threadIdx.x, k);
+  const double k = clip_factor<MAX>(raw, max_norm, grad_scale, stats, blockIdx.x == 0 && threadIdx.x == 0);
+  if (fits32(k)) {
+    for (int c = n_chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) scale_any<NT>(chunks[c], threadIdx.x, (float)k);
+  } else {
+    const FarFactor far = far_factor(k);
+    for (int c = n_chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) scale_any<NT>(chunks[c], threadIdx.x, far);
+  }
 }
 
 // Short lists (at most CLIP_SMALL_CHUNKS chunks of CLIP_SMALL_CHUNK elements): one workgroup, one launch.  Teams of two waves
@@ -364,8 +389,19 @@ __global__ __launch_bounds__(CLIP_SMALL_T * CLIP_SMALL_TEAMS) void norm_clip_ker
   }
   const double raw =
       block_combine<MAX, CLIP_SMALL_T * CLIP_SMALL_TEAMS>(MAX ? (double)__uint_as_float(acc.mx) : acc.sum, red);
-  const float k = clip_factor<MAX>(raw, max_norm, grad_scale, stats, threadIdx.x == 0);
+  const double kd = clip_factor<MAX>(raw, max_norm, grad_scale, stats, threadIdx.x == 0);
   if (!writes) return;
+  float k = (float)kd;
+  if (!fits32(kd)) {
+    k = 1.0f;
+    const FarFactor far = far_factor(kd);
+#pragma unroll
+    for (int u = 0; u < CLIP_SMALL_U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[u].f[i] = scaled(v[u].f[i], far);
+      tail[u] = scaled(tail[u], far);
+    }
+  }
 #pragma unroll
   for (int u = 0; u < CLIP_SMALL_U; ++u) {
     const unsigned td = ck[u].types >> 8, groups = ck[u].n / CLIP_E, i = groups * CLIP_E + t;

@@ -220,3 +220,36 @@ def test_captured_and_replayed_and_on_two_streams():
             got.append(norm_only.run(0.01))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("types", [[F32], [BF16], [BF16, F32]])
+@pytest.mark.parametrize("sizes,value,max_norm", [([5], 1e38, 0.01), ([100, 3], 1e38, 1e-4), ([300_001, 7], 1e38, 0.01),
+                                                  ([1_000_003, 17], 3e38, 0.01), ([1_000_003, 17], 3e38, 1e-7), ([40], 3e38, 1e-12)])
+def test_factors_below_the_normal_range_of_32_bits(types, sizes, value, max_norm):
+    """Gradients so large that the factor is far below 2^-126: it keeps its digits, into fp32 and in place.  The
+    factor's leading digits and the product are rounded to 24 digits each and scaled by a power of two (half a smallest step
+    where that leaves the normal range), so the bound of the other tests holds."""
+    src = [(torch.arange(n, device="cuda") % 7 - 3.0).div_(3.0).mul_(value).to(types[i % len(types)]) for i, n in enumerate(sizes)]
+    src[0][0] = value                                                                   # (never all zero)
+    keep = [t.clone() for t in src]
+    for norm in (2, math.inf):
+        want = reference(keep, max_norm, norm, 1.0)
+        assert 0 < want[2] < 2.0 ** -126
+        out = [torch.empty(n, device="cuda") for n in sizes]
+        stats = T.GradientClip(src, out=out).run(max_norm, norm=norm)
+        check_stats(stats, want, norm == math.inf)
+        check_out(out, keep, want[2])
+    T.GradientClip(src).run(max_norm)
+    check_out(src, keep, reference(keep, max_norm, 2, 1.0)[2])
+
+
+@pytest.mark.parametrize("sizes", [[11], [300_001, 7]])
+@pytest.mark.parametrize("value,grad_scale", [(1e-30, 2.0 ** 160), (2.0 ** -149, 2.0 ** 200), (3e38, 2.0 ** -200), (1.0, 1e-60), (3e38, 2.0 ** -270),
+                                              (2.0 ** -120, 3e70)])
+def test_scales_outside_the_range_of_32_bits(sizes, value, grad_scale):
+    """grad_scale may be any positive finite number of 64 bits; the scaled gradients are what 64 bits give, rounded to fp32."""
+    src = [torch.full((n,), value, device="cuda") for n in sizes]
+    out = [torch.empty(n, device="cuda") for n in sizes]
+    stats = T.GradientClip(src, out=out).run(0.0, grad_scale=grad_scale)
+    assert float(stats[2]) == grad_scale
+    check_out(out, src, grad_scale)
