@@ -513,7 +513,11 @@ int jirf_train_grad_clip_plan_create(int n, const void* const* src, const int* s
     const long step = CLIP_T * CLIP_E * CLIP_U;
     const long chunk = plan->small ? CLIP_SMALL_CHUNK
                                    : std::min<long>(65536, std::max<long>(step, (total / (4 * CLIP_MAX_BLOCKS) + step - 1) / step * step));
+    long n_chunks = 0;
+    for (int i = 0; i < n; ++i) n_chunks += (count[i] + chunk - 1) / chunk;
+    JIRF_REQUIRE(n_chunks < 1l << 26, JIRF_EINVAL, "grad_clip_plan_create: too many elements");
     std::vector<ClipChunk> chunks;
+    chunks.reserve(std::max(1l, n_chunks));
     for (int i = 0; i < n; ++i) {
       const int ts = type_of(src_dtype[i]), td = dst ? type_of(dst_dtype[i]) : TY_F32;
       for (long o = 0; o < count[i]; o += chunk)
@@ -524,7 +528,6 @@ int jirf_train_grad_clip_plan_create(int n, const void* const* src, const int* s
       if (dst) plan->bytes_written += (double)count[i] * type_bytes(td);
     }
     if (chunks.empty()) chunks.push_back({nullptr, nullptr, 0, 0});      // nothing to read, but a row for the kernel
-    JIRF_REQUIRE(chunks.size() < (size_t)1 << 30, JIRF_EINVAL, "grad_clip_plan_create: too many elements");
     JIRF_HIP_CHECK(hipGetDevice(&plan->device));
     plan->total = total;
     plan->writes = dst != nullptr;

@@ -194,3 +194,13 @@ def test_parameter_gradients_of_more_channels_than_a_grid_holds_are_refused(layo
     if not torch.cuda.is_available():        # nothing to launch on: the arguments themselves are taken
         assert bwd(**dict(kw, dpre_w=None)) != EINVAL
         assert bwd(**dict(kw, C=2**26 - 16)) != EINVAL
+
+
+def test_a_clip_plan_of_more_elements_than_any_memory_is_refused_before_its_table():
+    """2^46 elements would take 2^30 chunks, a table of 25 GB on the host; from 2^26 chunks on they are refused by their
+    number, with no table made."""
+    import resource
+    before = resource.getrusage(resource.RUSAGE_SELF).ru_maxrss
+    for src, count in (([A], [2**42]), ([A], [2**46]), ([A, A], [2**45, 2**45]), ([A], [2**62]), ([A] * 3, [2**45, 1, 2**45])):
+        assert plan(src, [0] * len(src), None, None, count) == EINVAL and "grad_clip" in jirf_hip.last_error()
+    assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 1 << 20        # (KiB)
