@@ -972,6 +972,12 @@ unsigned sweep_blocks(bool tok, int B, int P) {
   return (unsigned)std::min<long>(tiles, 1 << 16);
 }
 
+// A form that choose_form gives and no kernel is built for would leave the outputs unwritten: an error instead.
+[[noreturn]] inline void no_kernel(const RnForm& f) {
+  set_error("residual_norm: no %s kernel of %d lanes and %d vectors", f.tok ? "token" : "planar", f.lanes, f.nv);
+  throw Failure{JIRF_EINVAL};
+}
+
 #define RN_FWD_NT(TOK, L, NV, NT)                                                                                         \
   hipLaunchKernelGGL((rn_fwd_tile<T, TOK, L, NV, rn_vec<T>(TOK), NT>), dim3(f.blocks), dim3(f.threads), 0, s, a)
 #define RN_FWD(TOK, L, NV) RN_FWD_NT(TOK, L, NV, 0)
@@ -988,7 +994,7 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
       case 16: RN_FWD(true, 16, E8); break;
       case 32: RN_FWD(true, 32, E8); break;
       case 64: RN_FWD(true, 64, E8); break;
-      default:
+      case 0:
         if (f.nv == E8) {
           if (f.stream == 2) RN_FWD_NT(true, 0, E8, 2);
           else if (f.stream) RN_FWD_NT(true, 0, E8, 1);
@@ -998,6 +1004,8 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
           else if (f.stream) RN_FWD_NT(true, 0, 2 * E8, 1);
           else RN_FWD(true, 0, 2 * E8);
         }
+        break;
+      default: no_kernel(f);
     }
   } else {
     if constexpr (sizeof(T) == 4) {
@@ -1005,7 +1013,8 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
         switch (f.lanes) {
           case 2: RN_FWD(false, 2, 8); break;
           case 4: RN_FWD(false, 4, 8); break;
-          default: RN_FWD(false, 8, 8);
+          case 8: RN_FWD(false, 8, 8); break;
+          default: no_kernel(f);
         }
         return;
       }
@@ -1013,11 +1022,13 @@ void launch_fwd(const RnArgs& a, const RnForm& f, hipStream_t s) {
     switch (f.lanes) {
       case 2:
         if constexpr (sizeof(T) == 2) RN_FWD(false, 2, 4);
+        else no_kernel(f);
         break;
       case 4: RN_FWD(false, 4, 4); break;
       case 8: RN_FWD(false, 8, 4); break;
       case 16: RN_FWD(false, 16, 4); break;
-      default: RN_FWD(false, 32, 4);
+      case 32: RN_FWD(false, 32, 4); break;
+      default: no_kernel(f);
     }
   }
 }
@@ -1037,11 +1048,13 @@ void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
       case 16: RN_BWD(true, 16, E8); break;
       case 32: RN_BWD(true, 32, E8); break;
       case 64: RN_BWD(true, 64, E8); break;
-      default:
+      case 0:
         if (f.nv == E8 && f.stream) RN_BWD_NT(true, 0, E8, 1);
         else if (f.nv == E8) RN_BWD(true, 0, E8);
         else if (f.stream) RN_BWD_NT(true, 0, 2 * E8, 1);
         else RN_BWD(true, 0, 2 * E8);
+        break;
+      default: no_kernel(f);
     }
   } else {
     switch (f.lanes) {
@@ -1049,7 +1062,8 @@ void launch_bwd_tile(const RnArgs& a, const RnForm& f, hipStream_t s) {
       case 4: RN_BWD(false, 4, 4); break;
       case 8: RN_BWD(false, 8, 4); break;
       case 16: RN_BWD(false, 16, 4); break;
-      default: RN_BWD(false, 32, 4);
+      case 32: RN_BWD(false, 32, 4); break;
+      default: no_kernel(f);
     }
   }
 }

@@ -204,3 +204,21 @@ def test_a_clip_plan_of_more_elements_than_any_memory_is_refused_before_its_tabl
     for src, count in (([A], [2**42]), ([A], [2**46]), ([A, A], [2**45, 2**45]), ([A], [2**62]), ([A] * 3, [2**45, 1, 2**45])):
         assert plan(src, [0] * len(src), None, None, count) == EINVAL and "grad_clip" in jirf_hip.last_error()
     assert resource.getrusage(resource.RUSAGE_SELF).ru_maxrss - before < 1 << 20        # (KiB)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: only where there is nothing to launch on")
+@pytest.mark.parametrize("dtype", [0, 4, 5])
+@pytest.mark.parametrize("layout", [0, 1])
+def test_every_size_has_a_kernel(dtype, layout):
+    """Sizes on both sides of every choice of form: the arguments are taken and a kernel is found for them (the launch itself
+    fails, without a device).  A form without a kernel is an error, never a call that does nothing."""
+    Cs = sorted({c + d for c in (1, 4, 8, 16, 32, 64, 128, 256, 512, 1024, 2048, 4096, 8192, 16384) for d in (-1, 0, 1) if c + d > 0})
+    for C_ in Cs:
+        for P in (1, 2, 3, 4, 5, 7, 8, 9, 16, 31, 33, 64, 130, 1000, 8200, 300_001):
+            for B in (1, 3, 300):
+                b = dict(dtype=dtype, layout=layout, B=B, C=C_, P=P)
+                far = dict(x=1 << 44, f=2 << 44, y=3 << 44)
+                assert fwd(**b, **far) != EINVAL, (b, jirf_hip.last_error())
+                far = dict(dy=1 << 44, f=2 << 44, dx=3 << 44, df=4 << 44)
+                for gate in ({}, dict(gate_kind=1, gate=A), dict(gate_kind=2, gate=A)):
+                    assert bwd(**b, **far, **gate) != EINVAL, (b, gate, jirf_hip.last_error())
