@@ -300,7 +300,8 @@ struct Tile {
 #pragma unroll
     for (int s = 0; s < NS; ++s) rs[s] = recip_sqrt(fmaf(rs[s], inv, a.eps));
   }
-  // images [b0, b1) of worker w, and its first tile in each: it takes every a.S-th from there
+  // Images [b0, b1) of worker w (none behind the last image), and its first tile in each: it takes every a.S-th from there.
+  // There are at least a.S tiles, so every worker of an image has one.
   __device__ __forceinline__ void range(long w, int& b0, int& b1, int& t0) const {
     if (a.S > 1) {
       b0 = (int)min(w / a.S, (long)a.B);
@@ -338,7 +339,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : !TOK && sizeof(T) == 2 ? RN_
   int b0, b1, t0;
   ti.range(ti.worker(), b0, b1, t0);
   const int t1 = a.tiles;
-  if (b0 >= b1 || t0 >= t1) return;           // (uniform over the threads of a worker, and a worker's barriers are its own)
+  if (b0 >= b1) return;                       // (uniform over the threads of a worker, and a worker's barriers are its own)
   float pw[NV][NP], pb[NV][NP], gw[NV][NP], gb[NV][NP];
   Vec xn[NV], fn[NV];
   if (PF) {
@@ -446,8 +447,7 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_bwd_tile(const
   Ti ti(a, lds);
   int b0, b1, t0;
   ti.range(ti.worker(), b0, b1, t0);
-  const int slab = t0, t1 = a.tiles;
-  if (t0 >= t1) b1 = b0;                                       // nothing to do, but its partial sums are written (zeros)
+  const int slab = t0, t1 = a.tiles;                           // (a worker behind the last image still writes its sums, zeros)
   float acc[RN_Q_N][NV][NP], img[2][NV][NP];                   // img: G1, G0 of the current image
 #pragma unroll
   for (int q = 0; q < RN_Q_N; ++q)
@@ -653,15 +653,6 @@ __global__ __launch_bounds__(TOK && L ? RN_LANE_T : RN_T) void rn_bwd_tile(const
           }
         }
     }
-  }
-  if (IG && a.S > 1 && a.part_gate && b0 >= b1) {
-    // a worker without tiles still owns a row of the gate's partial sums
-    const int b = (int)(ti.worker() / a.S);
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < NP; ++i)
-        if (b < a.B && ti.exists(j, i) && (TOK || ti.pl == 0)) a.part_gate[((long)b * a.S + slab) * a.C + ti.channel(j) + i] = 0.f;
   }
   if (!a.part) return;
   // one row of partial sums per workgroup, for the quantities that are wanted
