@@ -5,7 +5,8 @@ gradients as torch tensors; `jirf_hip.train.AstTrainStep` is the whole step for 
 
 Everything runs asynchronously on the current stream of the tensors' device and can be captured into a graph (plans are
 made outside a capture); workspaces come from torch's allocator per call, so calls on several streams do not share
-any.  There is no CPU path and no autograd graph: the backward is called by name, as everywhere in jirf_hip.train.
+any.  There is no CPU path and no autograd graph: the backward is called by name, as everywhere in jirf_hip.train, and tensors
+that require gradients are refused except under torch.no_grad().
 """
 from __future__ import annotations
 
@@ -53,10 +54,18 @@ def _sizes(x: torch.Tensor, layout: str):
     return B, Cn, P, lay, dtype
 
 
+def _refuse_tracked(name: str):
+    if torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and there is no autograd graph through these operators: detach it, or call "
+                         "under torch.no_grad() and take the gradients from the backward by name")
+
+
 def _bs(name: str, t: torch.Tensor, like: torch.Tensor) -> int:
     """Batch stride (0: dense) of an activation that has to match `like`."""
     if t is not like and (t.shape != like.shape or t.dtype is not like.dtype or t.get_device() != like.get_device()):
         raise ValueError(f"{name}: {tuple(t.shape)} {t.dtype} on {t.device}, expected {tuple(like.shape)} {like.dtype} on {like.device}")
+    if t.requires_grad:
+        _refuse_tracked(name)
     if t.is_contiguous():
         return 0
     bs = t.stride(0)
@@ -69,6 +78,8 @@ def _param(name: str, t: torch.Tensor, shape, like: torch.Tensor) -> int:
     if t.dtype is not torch.float32 or t.shape != shape or t.get_device() != like.get_device() or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous float32 tensor {shape} on {like.device} is needed, got {tuple(t.shape)} {t.dtype} "
                          f"on {t.device}")
+    if t.requires_grad:
+        _refuse_tracked(name)
     return t.data_ptr()
 
 

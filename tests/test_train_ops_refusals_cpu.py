@@ -222,3 +222,18 @@ def test_every_size_has_a_kernel(dtype, layout):
                 far = dict(dy=1 << 44, f=2 << 44, dx=3 << 44, df=4 << 44)
                 for gate in ({}, dict(gate_kind=1, gate=A), dict(gate_kind=2, gate=A)):
                     assert bwd(**b, **far, **gate) != EINVAL, (b, gate, jirf_hip.last_error())
+
+
+def test_python_layer_refuses_tensors_of_an_autograd_graph():
+    """There is no graph through these operators: outputs of tracked inputs would be cut off from it without a word."""
+    like = torch.zeros(3, 8, 6)
+    tracked, w = torch.zeros(3, 8, 6, requires_grad=True), torch.zeros(8, requires_grad=True)
+    calls = [lambda: T._bs("x", tracked, tracked), lambda: T._bs("branch", tracked * 2, like), lambda: T._gate(w, 3, 8, like),
+             lambda: T._gate(torch.zeros(3, 8, requires_grad=True), 3, 8, like), lambda: T._norm("pre", (1, w, None), 8, like),
+             lambda: T._norm("post", (1, torch.zeros(8), w), 8, like), lambda: T._param("scale", torch.zeros(3, requires_grad=True), (3,), like)]
+    for call in calls:
+        with pytest.raises(ValueError, match="no autograd graph"):
+            call()
+        with torch.no_grad():
+            call()
+    assert T._bs("x", tracked.detach(), like) == 0
