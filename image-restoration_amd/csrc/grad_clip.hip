@@ -462,7 +462,7 @@ void check_ranges(int n, const void* const* src, const int* sdt, void* const* ds
     r.push_back({d, d + (uintptr_t)count[i] * type_bytes(type_of(ddt[i])), i, true});
   }
   std::sort(r.begin(), r.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
-  // sweep: the furthest end so far of any source and of any destination, and of any by another tensor
+  // in the order of their starts, each range against the earlier ones that have not ended before it starts
   std::vector<const Range*> open;
   for (const Range& a : r) {
     size_t keep = 0;

@@ -136,8 +136,10 @@ __device__ __forceinline__ float lane_sum(float x) {
   }
   return x;
 }
-// 1 / sqrt(x), correctly rounded: the hardware's estimate and one Newton step whose residual 1 - x y^2 is formed without
-// rounding error (product and its remainder apart); small x scaled into the estimate's range, 0 and infinity as they are.
+// 1 / sqrt(x) within half a unit in the last place and 2^-21 of one: the hardware's estimate and one Newton step whose residual
+// 1 - x y^2 keeps the product's remainder.  Nearly always the nearest value: of the 2^24 in [1, 4), 1 to 7 get the other
+// neighbour, depending on which value within one unit the estimate is (2.1552868 from the nearest estimate, for one).  Small x are
+// scaled into the estimate's range, 0 and infinity are as they are.
 __device__ __forceinline__ float recip_sqrt(float x) {
   const bool tiny = x < 0x1p-96f;
   x *= tiny ? 0x1p64f : 1.0f;

@@ -150,9 +150,10 @@ def residual_norm_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], y:
                       gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, pre: Optional[Norm] = None,
                       layout: str = "planar") -> dict:
     """Gradients of residual_norm: {"dx", "dbranch", "dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b"}, None where
-    there is no such input.  dy: gradient of y (None: zero), dn: gradient of n; y, stats: the forward's; branch: the
-    forward's input (needed with a post norm or a gate).  Without a pre norm dx is dy itself, not a copy, and so is
-    dbranch where the branch has no norm, gate or scale either."""
+    there is no such input.  dy: gradient of y (None: zero), dn: gradient of n (not read without a pre norm: there is no
+    n); y, stats: the forward's; branch: the forward's input (needed with a post norm or a gate).  Without a pre norm dx is
+    dy itself, not a copy, and so is dbranch where the branch has no norm, gate or scale either: clone it before adding to
+    it in place."""
     like = dy if dy is not None else dn
     if like is None:
         raise ValueError("residual_norm_bwd: dy or dn is needed")
@@ -208,7 +209,8 @@ class GradientClip:
 
     tensors: contiguous float32 / bfloat16 / float16 tensors on one GPU, any number of elements (0 too).  out: None to clip
     in place, a list of as many tensors (any of the three types, e.g. slices of a flat float32 buffer), or False for the
-    norm alone.  The object keeps the tensors; make a new one when a gradient moves to other memory."""
+    norm alone.  The object keeps the tensors; make a new one when a gradient moves to other memory.  It is made and dropped
+    outside captures, and kept as long as a graph that holds one of its runs: every replay reads its table."""
 
     def __init__(self, tensors: Sequence[torch.Tensor], out=None):
         self._plan = None
