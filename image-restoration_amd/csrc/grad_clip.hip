@@ -16,8 +16,8 @@
 //
 // Bound by memory: the gradients are read twice and written once (the second reading starts with what the cache still
 // holds).  Measured a call: 282 fp32 tensors of 26.3 M values into a flat buffer 54 us (316 MB, 5.8 TB/s; the copy of a
-// large buffer reaches 4.8), 401 tensors of three types and 60 M values to fp32 107 us, 536 M bf16 595 us (3.2 GB,
-// 5.4 TB/s); 24 tensors of 40 k values 7.3 us in one launch (two launches: 12.4).
+// large buffer reaches 4.8), 401 tensors of three types and 60 M values to fp32 107 us, 536 M bf16 593 us (3.2 GB,
+// 5.4 TB/s); 24 tensors of 40 k values 7.4 us in one launch (two launches: 12.4).
 #include <algorithm>
 #include <cmath>
 #include <memory>
